@@ -420,6 +420,119 @@ int pi_tq_attn_decode(pi_handle h, const float* d_q, pi_tq_pool pool, const int3
                       int32_t n_q_heads, int32_t gqa_mode, const float* d_gate, float* d_out,
                       void* stream);
 
+/* ---- rotary plans --------------------------------------------------------------------
+ * Rotary positions beyond pi_rope's (which keeps the reference's f32 formula, src/ops.rs:35-157):
+ * frequencies scaled for long contexts, angles reduced in 64 bits (exact at any int32 position),
+ * f32 / f16 / bf16 rows at their own strides, in place or into another tensor.  Channel pair i of
+ * rope_dim / 2 is (2i, 2i+1) or (i, i + rope_dim/2); the channels past rope_dim pass through.
+ *   y0 = m (x0 cos a - x1 sin a),  y1 = m (x0 sin a + x1 cos a),  a = position * freq_i  */
+typedef struct pi_rope_plan_s* pi_rope_plan;
+typedef enum pi_rope_layout { PI_ROPE_PAIRS = 0, PI_ROPE_HALVES = 1 } pi_rope_layout;
+/* freq_i from base^(-2i / rope_dim) and the parameters in brackets, all above 0:
+ *   PLAIN   []                              unscaled
+ *   LINEAR  [factor]                        freq / factor
+ *   NTK     [factor]                        base * factor^(rope_dim / (rope_dim - 2))
+ *   YARN    [factor, orig, fast, slow]      pairs that turn at least `fast` times in a context of
+ *                                           `orig` tokens keep their frequency, those that turn at most
+ *                                           `slow` times get freq / factor, a linear ramp over the pair
+ *                                           index between (whole indices); m = 0.1 ln(factor) + 1
+ *   BANDS   [factor, orig, low, high]       freq / factor below `low` turns in `orig` tokens, freq above
+ *                                           `high`, linear in the turns between; high > low */
+typedef enum pi_rope_scaling {
+    PI_ROPE_PLAIN = 0, PI_ROPE_LINEAR = 1, PI_ROPE_NTK = 2, PI_ROPE_YARN = 3, PI_ROPE_BANDS = 4
+} pi_rope_scaling;
+/* Host only: rope_dim / 2 frequencies and m (rope_dim even).  Errors through pi_last_error(NULL). */
+int pi_rope_scaled_freqs(int32_t rope_dim, double base, int32_t scaling, const double* h_params,
+                         int32_t n_params, double* h_freqs, double* h_mscale);
+/* A plan of any frequencies (rope_dim even, 2..256), kept on the device. */
+int pi_rope_plan_create(pi_handle h, int32_t rope_dim, int32_t layout, const double* h_freqs,
+                        double mscale, pi_rope_plan* out);
+/* Waits for all work on the device first. */
+void pi_rope_plan_destroy(pi_rope_plan plan);
+/* Rotates q, and k unless d_k is NULL, at positions d_pos[n_tok].  Element (token t, head h, channel d) of
+ * a tensor lies at t * tok + h * head + d, strides in elements (any order and alignment; rows of 16-byte
+ * aligned chunks take the vector kernel).  An output is either its input with the same
+ * strides (in place) or shares no memory with it. */
+int pi_rope_apply(pi_handle h, pi_rope_plan plan, int32_t dtype, int32_t n_tok, int32_t head_dim,
+                  const int32_t* d_pos, const void* d_q, int64_t q_tok, int64_t q_head,
+                  int32_t n_q_heads, void* d_q_out, int64_t qo_tok, int64_t qo_head, const void* d_k,
+                  int64_t k_tok, int64_t k_head, int32_t n_kv_heads, void* d_k_out, int64_t ko_tok,
+                  int64_t ko_head, void* stream);
+
+/* ---- KV cache held in 4 bits -----------------------------------------------------------
+ * Keys and values in 16-token pages like pi_kv_pool's, in groups of 32 channels of one token's head:
+ *   m     the group's value of largest magnitude (the positive one of a tie)
+ *   s     -m / 8 to 7 significant bits, nearest even (a multiple of 2^-20 below 2^-14), |s| <= 904; f16
+ *   code  clamp(rint(x / s), -8, 7) + 8, or 8 where s is 0;  value s * (code - 8)
+ * 4.5 bits a value: 9/32 of an f16 pool.  Values are exact in f16 and finite: magnitudes past 7232 and
+ * infinities saturate, a NaN counts as 0 (the queries still carry one), and unwritten slots are 0, so a masked
+ * key can never spoil a row.  head_dim 64, 128 or 256, page_tokens 16.
+ * Device tables are read, not trusted: a position past the page-table row or on a page id outside
+ * [0, n_pages) is neither stored nor attended, negative start positions count as 0. */
+typedef struct pi_q4_pool_s* pi_q4_pool;
+int pi_q4_pool_create(pi_handle h, int32_t n_pages, int32_t page_tokens, int32_t n_kv_heads,
+                      int32_t head_dim, pi_q4_pool* out);
+/* Waits for all work on the device first. */
+void pi_q4_pool_destroy(pi_q4_pool pool);
+size_t pi_q4_pool_bytes(pi_q4_pool pool);
+/* The prologue of an attention step over this cache in one launch (as pi_attn_prologue, src/model/mod.rs:
+ * 1035-1146): per-head RMSNorm of q and k (d_q_norm_w, d_k_norm_w f32 [head_dim], NULL: none), rotation by
+ * `plan` (NULL: none) at each token's position, q written to d_q_out, k and v quantised into the pages.
+ * The n_rows tokens are a ragged batch: sequence s holds rows d_tok_start[s] .. d_tok_start[s + 1] - 1
+ * (device int32 [n_seq + 1], non-decreasing) at positions d_start_pos[s] ...; NULL: row s is sequence s's one
+ * token (n_rows = n_seq).  Rows of no sequence are neither read nor written anywhere.  Inputs as in
+ * pi_rope_apply (strides in elements); d_q may be NULL (k and v alone); d_q_out shares no memory with the
+ * inputs.  d_k_values, d_v_values (each NULL or f16 [n_rows][n_kv_heads][head_dim], 16-byte aligned) receive the
+ * values that the cache now holds, for pi_attn_prefill over a fresh prompt.  n_seq <= 4096.  One call must not
+ * store two tokens in one slot (a page in two rows of the table is fine for reading). */
+int pi_q4_append(pi_handle h, pi_q4_pool pool, pi_rope_plan plan, int32_t dtype, int32_t n_rows,
+                 const int32_t* d_tok_start, const int32_t* d_start_pos, int32_t n_seq,
+                 const int32_t* d_page_table, int32_t max_pages, const void* d_q, int64_t q_tok,
+                 int64_t q_head, int32_t n_q_heads, void* d_q_out, int64_t qo_tok, int64_t qo_head,
+                 const void* d_k, int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok,
+                 int64_t v_head, const float* d_q_norm_w, const float* d_k_norm_w, float eps,
+                 uint16_t* d_k_values, uint16_t* d_v_values, void* stream);
+/* The records of positions start .. start + n_tok - 1 of sequence `seq`, out of the pages and back into them:
+ * codes [n_tok][n_kv_heads][head_dim / 2] (even channel in the low four bits), scales
+ * [n_tok][n_kv_heads][head_dim / 32] as f16 bits.  Positions that no page holds read as zeros (code 8, scale
+ * 0).  pi_q4_write clears a scale's four low bits, limits it to 904 and takes a NaN as 0, so what was read is
+ * restored bit for bit and nothing else gets in. */
+int pi_q4_read(pi_handle h, pi_q4_pool pool, const int32_t* d_page_table, int32_t max_pages,
+               int32_t seq, int32_t start, int32_t n_tok, uint8_t* d_k_codes, uint16_t* d_k_scales,
+               uint8_t* d_v_codes, uint16_t* d_v_scales, void* stream);
+int pi_q4_write(pi_handle h, pi_q4_pool pool, const int32_t* d_page_table, int32_t max_pages,
+                int32_t seq, int32_t start, int32_t n_tok, const uint8_t* d_k_codes,
+                const uint16_t* d_k_scales, const uint8_t* d_v_codes, const uint16_t* d_v_scales,
+                void* stream);
+/* Attention over the cache (src/model/mod.rs:1148-1196): softmax(scale q.k) v over each row's keys, times
+ * sigmoid(gate) where d_gate is not NULL; f32 softmax and sums, q, gate and out all in dtype (f32, f16 or bf16;
+ * f32 rows keep f32 accuracy).  Head maps as pi_attn_decode.  A row without keys gets zeros.
+ * q, gate, out and the workspace are 16-byte aligned and contiguous.
+ * max_ctx: no sequence holds more tokens (0: 16 * max_pages); a longer one is cut to it, rounded up to whole
+ * pages.  A small max_ctx on a wide table saves a launch.
+ * The workspace is the caller's, of at least pi_q4_attn_ws_bytes for the same arguments (0: NULL will do; for
+ * a decode n_rows = n_seq and max_tok = 1), and belongs to the call until it has run.  The calls
+ * allocate nothing and hold nothing, so they can be captured; graphs or streams that may run at
+ * the same time need workspaces of their own. */
+int pi_q4_attn_ws_bytes(pi_handle h, pi_q4_pool pool, int32_t dtype, int32_t n_rows, int32_t n_seq,
+                        int32_t max_tok, int32_t max_pages, int32_t max_ctx, int32_t n_q_heads,
+                        int32_t gqa_mode, size_t* bytes);
+/* One token a sequence: q [batch][n_q_heads][head_dim] over d_ctx_len[b] cached tokens, its own among them
+ * (append first).  batch <= 4096. */
+int pi_q4_attn_decode(pi_handle h, pi_q4_pool pool, const void* d_q, int32_t dtype,
+                      const int32_t* d_page_table, int32_t max_pages, int32_t max_ctx,
+                      const int32_t* d_ctx_len, int32_t batch, int32_t n_q_heads, int32_t gqa_mode,
+                      float scale, const void* d_gate, void* d_out, void* d_ws, size_t ws_bytes,
+                      void* stream);
+/* A chunk of tokens a sequence, causal: rows as in pi_q4_append, row i of sequence s sees keys 0 ..
+ * d_start_pos[s] + i (its chunk appended first).  No sequence has more than max_tok rows; the rows of a
+ * longer one past max_tok, and rows of no sequence, are left as they were.  n_seq <= 4096. */
+int pi_q4_attn_prefill(pi_handle h, pi_q4_pool pool, const void* d_q, int32_t dtype, int32_t n_rows,
+                       const int32_t* d_tok_start, const int32_t* d_start_pos, int32_t n_seq,
+                       int32_t max_tok, const int32_t* d_page_table, int32_t max_pages,
+                       int32_t max_ctx, int32_t n_q_heads, int32_t gqa_mode, float scale,
+                       const void* d_gate, void* d_out, void* d_ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

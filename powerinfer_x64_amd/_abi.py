@@ -17,6 +17,8 @@ LIB_PATH = os.environ.get("PI_ATTN_LIB") or os.path.join(
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
+_i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 _int = ctypes.c_int
 
@@ -83,6 +85,25 @@ SIGNATURES = {
     "pi_tq_append": (_int, [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp]),
     "pi_tq_read": (_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "pi_tq_attn_decode": (_int, [_vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "pi_rope_scaled_freqs": (_int, [_i32, _f64, _i32, _vp, _i32, _vp, _vp]),
+    "pi_rope_plan_create": (_int, [_vp, _i32, _i32, _vp, _f64, ctypes.POINTER(_vp)]),
+    "pi_rope_plan_destroy": (None, [_vp]),
+    "pi_rope_apply": (_int, [_vp, _vp, _i32, _i32, _i32, _vp, _vp, _i64, _i64, _i32, _vp, _i64, _i64,
+                             _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp]),
+    "pi_q4_pool_create": (_int, [_vp, _i32, _i32, _i32, _i32, ctypes.POINTER(_vp)]),
+    "pi_q4_pool_destroy": (None, [_vp]),
+    "pi_q4_pool_bytes": (_sz, [_vp]),
+    "pi_q4_append": (_int, [_vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _vp, _i32, _vp, _i64, _i64,
+                            _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _f32,
+                            _vp, _vp, _vp]),
+    "pi_q4_read": (_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "pi_q4_write": (_int, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "pi_q4_attn_ws_bytes": (_int, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                   ctypes.POINTER(_sz)]),
+    "pi_q4_attn_decode": (_int, [_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _f32,
+                                 _vp, _vp, _vp, _sz, _vp]),
+    "pi_q4_attn_prefill": (_int, [_vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i32,
+                                  _i32, _i32, _f32, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

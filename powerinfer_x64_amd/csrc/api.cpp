@@ -6,6 +6,7 @@
 // an exception or an abort across the ABI.
 #include "pi_attn.h"
 #include "pi_launch.hpp"
+#include "q4_launch.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -82,6 +83,17 @@ struct pi_gdn_layer_s {
     float* d_state = nullptr;       // [hv][dk][dv]
     float* d_buf = nullptr;         // staging: activation, q, k, v, beta, g (+ host-slice I/O)
     size_t buf_floats = 0;
+};
+
+struct pi_rope_plan_s {
+    pi_handle owner;
+    pi::RopePlan p;
+};
+
+struct pi_q4_pool_s {
+    pi_handle owner;
+    pi::Q4Geom g;
+    size_t bytes;
 };
 
 struct pi_tq_pool_s {
@@ -1848,6 +1860,385 @@ int pi_tq_attn_decode(pi_handle h, const float* d_q, pi_tq_pool pool, const int3
                                              d_gate, d_out, plan);
     PI_HIP(h, pi::launch_decode(g, p, h->dws, plan, s), "pi_tq_attn_decode");
     return ws_end(h, s, "pi_tq_attn_decode");
+}
+
+// ---- rotary plans ----------------------------------------------------------------
+
+namespace {
+// Makes a handle's device current and puts the caller's back at the end.
+struct DeviceScope {
+    int old = -1;
+    hipError_t err = hipSuccess;
+    explicit DeviceScope(int device) {
+        err = hipGetDevice(&old);
+        if (err != hipSuccess || old == device) {
+            old = -1;
+            if (err == hipSuccess) return;
+        }
+        err = hipSetDevice(device);
+    }
+    ~DeviceScope() {
+        if (old >= 0) (void)hipSetDevice(old);
+    }
+};
+
+// Rows (t, h) of a written tensor must not share elements.
+bool rows_disjoint(int64_t tok, int64_t head, int32_t n_tok, int32_t n_heads, int32_t dim) {
+    if (n_tok <= 1) return n_heads <= 1 || head >= dim;
+    if (n_heads <= 1) return tok >= dim;
+    const bool head_in = head <= tok;
+    const int64_t lo = head_in ? head : tok, hi = head_in ? tok : head, n = head_in ? n_heads : n_tok;
+    return lo >= dim && hi >= (n - 1) * lo + dim;
+}
+
+int dtype_bytes(int32_t dtype) { return dtype == PI_F32 ? 4 : 2; }
+}  // namespace
+
+int pi_rope_scaled_freqs(int32_t rope_dim, double base, int32_t scaling, const double* params, int32_t n_params, double* freqs,
+                         double* mscale) {
+    if (!freqs || !mscale) return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: null output");
+    if (rope_dim < 2 || rope_dim % 2 || !(base > 0) || !std::isfinite(base))
+        return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: rope_dim=%d base=%g", rope_dim, base);
+    const int32_t want[] = {0, 1, 1, 4, 4};
+    if (scaling < PI_ROPE_PLAIN || scaling > PI_ROPE_BANDS)
+        return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: scaling %d", scaling);
+    if (n_params != want[scaling] || (n_params && !params))
+        return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: scaling %d takes %d parameters (got %d)", scaling,
+                    want[scaling], n_params);
+    for (int32_t i = 0; i < n_params; ++i)
+        if (!(params[i] > 0) || !std::isfinite(params[i]))
+            return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: parameter %d is %g", i, params[i]);
+    if (scaling == PI_ROPE_NTK && rope_dim == 2)
+        return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: ntk needs rope_dim > 2");
+    if (scaling == PI_ROPE_YARN && base == 1.0)
+        return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: yarn needs a base other than 1");
+    if (scaling == PI_ROPE_BANDS && !(params[3] > params[2]))
+        return fail(nullptr, PI_ERR_INVALID_ARG, "pi_rope_scaled_freqs: bands needs high > low (got %g, %g)", params[3], params[2]);
+    const double dim = rope_dim, factor = n_params ? params[0] : 1.0;
+    if (scaling == PI_ROPE_NTK) base *= std::pow(factor, dim / (dim - 2));
+    double lo = 0, hi = 0;
+    if (scaling == PI_ROPE_YARN) {
+        const auto at = [&](double turns) { return dim * std::log(params[1] / (turns * 2 * M_PI)) / (2 * std::log(base)); };
+        lo = std::max(std::floor(at(params[2])), 0.0);
+        hi = std::min(std::ceil(at(params[3])), dim - 1);
+    }
+    for (int32_t i = 0; i < rope_dim / 2; ++i) {
+        const double f = std::pow(base, -2.0 * i / dim);
+        double r = 1.0;  // share of the unscaled frequency
+        if (scaling == PI_ROPE_LINEAR) r = 0.0;
+        if (scaling == PI_ROPE_YARN) r = 1.0 - std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 0.001)));
+        if (scaling == PI_ROPE_BANDS)
+            r = std::min(1.0, std::max(0.0, (params[1] * f / (2 * M_PI) - params[2]) / (params[3] - params[2])));
+        freqs[i] = f / factor * (1 - r) + f * r;
+        if (scaling == PI_ROPE_NTK) freqs[i] = f;
+    }
+    *mscale = scaling == PI_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    return PI_OK;
+}
+
+int pi_rope_plan_create(pi_handle h, int32_t rope_dim, int32_t layout, const double* freqs, double mscale, pi_rope_plan* out) {
+    PI_CHECK_HANDLE(h);
+    if (!out) return fail(h, PI_ERR_INVALID_ARG, "pi_rope_plan_create: out is null");
+    *out = nullptr;
+    if (!freqs) return fail(h, PI_ERR_INVALID_ARG, "pi_rope_plan_create: freqs is null");
+    if (rope_dim < 2 || rope_dim % 2 || rope_dim > 256)
+        return fail(h, PI_ERR_UNSUPPORTED, "pi_rope_plan_create: rope_dim %d (even, 2..256)", rope_dim);
+    if (layout != PI_ROPE_PAIRS && layout != PI_ROPE_HALVES)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_plan_create: layout %d", layout);
+    if (!std::isfinite(mscale)) return fail(h, PI_ERR_INVALID_ARG, "pi_rope_plan_create: mscale %g", mscale);
+    double turns[128];
+    for (int32_t i = 0; i < rope_dim / 2; ++i) {
+        if (!std::isfinite(freqs[i])) return fail(h, PI_ERR_INVALID_ARG, "pi_rope_plan_create: frequency %d is %g", i, freqs[i]);
+        turns[i] = freqs[i] / (2 * M_PI);
+    }
+    const DeviceScope on(h->device);
+    PI_HIP(h, on.err, "pi_rope_plan_create");
+    pi_rope_plan p = new (std::nothrow) pi_rope_plan_s();
+    if (!p) return fail(h, PI_ERR_OUT_OF_MEMORY, "pi_rope_plan_create: host allocation");
+    p->owner = h;
+    p->p = pi::RopePlan{nullptr, rope_dim / 2, layout, mscale};
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&p->p.turns), sizeof turns);
+    if (e == hipSuccess) e = hipMemcpy(p->p.turns, turns, sizeof(double) * (rope_dim / 2), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        (void)hipFree(p->p.turns);
+        delete p;
+        return hip_fail(h, e, "pi_rope_plan_create");
+    }
+    *out = p;
+    return PI_OK;
+}
+
+void pi_rope_plan_destroy(pi_rope_plan plan) {
+    if (!plan) return;
+    const DeviceScope on(plan->owner->device);
+    (void)hipDeviceSynchronize();
+    (void)hipFree(plan->p.turns);
+    delete plan;
+}
+
+int pi_rope_apply(pi_handle h, pi_rope_plan plan, int32_t dtype, int32_t n_tok, int32_t head_dim, const int32_t* d_pos,
+                  const void* d_q, int64_t q_tok, int64_t q_head, int32_t n_q_heads, void* d_q_out, int64_t qo_tok, int64_t qo_head,
+                  const void* d_k, int64_t k_tok, int64_t k_head, int32_t n_kv_heads, void* d_k_out, int64_t ko_tok, int64_t ko_head,
+                  void* stream) {
+    PI_CHECK_HANDLE(h);
+    if (!plan) return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: null argument");
+    if (plan->owner->device != h->device)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: the plan is on device %d", plan->owner->device);
+    if (n_tok == 0) return PI_OK;  // empty tensors have no address
+    if (!d_q || !d_q_out || !d_pos || (d_k && !d_k_out))
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: null argument");
+    if (!d_k) n_kv_heads = 0;
+    if (dtype < PI_F32 || dtype > PI_BF16) return fail(h, PI_ERR_UNSUPPORTED, "pi_rope_apply: dtype %d", dtype);
+    if (n_tok < 0 || n_q_heads <= 0 || n_kv_heads < (d_k ? 1 : 0) || n_q_heads > 65536 || n_kv_heads > 65536)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: n_tok=%d heads=%d/%d", n_tok, n_q_heads, n_kv_heads);
+    if (head_dim < 2 * plan->p.half || head_dim > 65536)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: head_dim %d for a plan of %d channels", head_dim, 2 * plan->p.half);
+    if (q_tok < 0 || q_head < 0 || (d_k && (k_tok < 0 || k_head < 0)))
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: negative stride");
+    if (!rows_disjoint(qo_tok, qo_head, n_tok, n_q_heads, head_dim) ||
+        (d_k && !rows_disjoint(ko_tok, ko_head, n_tok, n_kv_heads, head_dim)))
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: output rows overlap");
+    if ((d_q == d_q_out && (q_tok != qo_tok || q_head != qo_head)) || (d_k && d_k == d_k_out && (k_tok != ko_tok || k_head != ko_head)))
+        return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: in place needs the output's strides");
+    const DeviceScope on(h->device);
+    PI_HIP(h, on.err, "pi_rope_apply");
+    pi::RopeArgs a{};
+    a.plan = plan->p;
+    a.in[0] = {const_cast<void*>(d_q), q_tok, q_head, n_q_heads};
+    a.out[0] = {d_q_out, qo_tok, qo_head, n_q_heads};
+    a.in[1] = {const_cast<void*>(d_k), k_tok, k_head, n_kv_heads};
+    a.out[1] = {d_k_out, ko_tok, ko_head, n_kv_heads};
+    a.pos = d_pos;
+    a.n_tok = n_tok;
+    a.head_dim = head_dim;
+    a.dtype = dtype;
+    PI_HIP(h, pi::launch_rope_apply(a, pick(h, stream)), "pi_rope_apply");
+    return PI_OK;
+}
+
+// ---- 4-bit cache -------------------------------------------------------------------
+
+int pi_q4_pool_create(pi_handle h, int32_t n_pages, int32_t page_tokens, int32_t n_kv_heads, int32_t head_dim, pi_q4_pool* out) {
+    PI_CHECK_HANDLE(h);
+    if (!out) return fail(h, PI_ERR_INVALID_ARG, "pi_q4_pool_create: out is null");
+    *out = nullptr;
+    if (page_tokens != pi::kPageTokens)
+        return fail(h, PI_ERR_UNSUPPORTED, "pi_q4_pool_create: page_tokens must be 16 (got %d)", page_tokens);
+    if (n_pages <= 0 || n_kv_heads <= 0)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_pool_create: n_pages=%d n_kv_heads=%d", n_pages, n_kv_heads);
+    if (!dim_ok(head_dim)) return fail(h, PI_ERR_UNSUPPORTED, "pi_q4_pool_create: head_dim %d (64/128/256)", head_dim);
+    const DeviceScope on(h->device);
+    PI_HIP(h, on.err, "pi_q4_pool_create");
+    pi_q4_pool p = new (std::nothrow) pi_q4_pool_s();
+    if (!p) return fail(h, PI_ERR_OUT_OF_MEMORY, "pi_q4_pool_create: host allocation");
+    p->owner = h;
+    p->bytes = (size_t)n_pages * n_kv_heads * pi::q4_block_bytes(head_dim);
+    void* base = nullptr;
+    hipError_t e = hipMalloc(&base, p->bytes);
+    if (e == hipSuccess) e = hipMemset(base, 0, p->bytes);  // scales of 0: unwritten slots hold zeros
+    if (e != hipSuccess) {
+        (void)hipFree(base);
+        delete p;
+        return hip_fail(h, e, "pi_q4_pool_create");
+    }
+    p->g = pi::Q4Geom{static_cast<char*>(base), n_pages, n_kv_heads, head_dim};
+    *out = p;
+    return PI_OK;
+}
+
+void pi_q4_pool_destroy(pi_q4_pool pool) {
+    if (!pool) return;
+    const DeviceScope on(pool->owner->device);
+    (void)hipDeviceSynchronize();
+    (void)hipFree(pool->g.base);
+    delete pool;
+}
+
+size_t pi_q4_pool_bytes(pi_q4_pool pool) { return pool ? pool->bytes : 0; }
+
+int pi_q4_append(pi_handle h, pi_q4_pool pool, pi_rope_plan plan, int32_t dtype, int32_t n_rows, const int32_t* d_tok_start,
+                 const int32_t* d_start_pos, int32_t n_seq, const int32_t* d_page_table, int32_t max_pages, const void* d_q,
+                 int64_t q_tok, int64_t q_head, int32_t n_q_heads, void* d_q_out, int64_t qo_tok, int64_t qo_head, const void* d_k,
+                 int64_t k_tok, int64_t k_head, const void* d_v, int64_t v_tok, int64_t v_head, const float* d_q_norm_w,
+                 const float* d_k_norm_w, float eps, uint16_t* d_k_values, uint16_t* d_v_values, void* stream) {
+    PI_CHECK_HANDLE(h);
+    if (!pool) return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: null argument");
+    const pi::Q4Geom& g = pool->g;
+    if (n_rows == 0 && n_seq >= 0) return PI_OK;  // empty tensors have no address
+    if (!d_k || !d_v || !d_start_pos || !d_page_table || (d_q && !d_q_out))
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: null argument");
+    if (!d_q) n_q_heads = 0;
+    if (dtype < PI_F32 || dtype > PI_BF16) return fail(h, PI_ERR_UNSUPPORTED, "pi_q4_append: dtype %d", dtype);
+    if (n_rows < 0 || n_seq < 0 || n_seq > pi::kQ4MaxBatch || max_pages <= 0 || max_pages > (1 << 26) || n_q_heads < (d_q ? 1 : 0) ||
+        n_q_heads > 65536)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: n_rows=%d n_seq=%d (at most %d) max_pages=%d n_q_heads=%d", n_rows, n_seq,
+                    pi::kQ4MaxBatch, max_pages, n_q_heads);
+    if (!d_tok_start && n_rows != n_seq)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: %d rows for %d sequences of one token each", n_rows, n_seq);
+    if (plan && 2 * plan->p.half > g.head_dim)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: a plan of %d channels for head_dim %d", 2 * plan->p.half, g.head_dim);
+    if (plan && plan->owner->device != h->device)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: the plan is on device %d", plan->owner->device);
+    if (pool->owner->device != h->device)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: the pool is on device %d", pool->owner->device);
+    if ((d_q && (q_tok < 0 || q_head < 0)) || k_tok < 0 || k_head < 0 || v_tok < 0 || v_head < 0)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: negative stride");
+    if (!(eps >= 0)) return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: eps %g", eps);
+    if (d_q) {
+        if (!rows_disjoint(qo_tok, qo_head, n_rows, n_q_heads, g.head_dim))
+            return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: output rows overlap");
+        if (d_q == d_q_out)  // a lane's partner channels would be read after they are written
+            return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: q_out must be another tensor than q");
+    }
+    if (reinterpret_cast<uintptr_t>(d_k_values) % 16 || reinterpret_cast<uintptr_t>(d_v_values) % 16)
+        return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: k_values / v_values must be 16-byte aligned");
+    if (n_seq == 0) return PI_OK;
+    const DeviceScope on(h->device);
+    PI_HIP(h, on.err, "pi_q4_append");
+    pi::Q4AppendArgs a{};
+    a.g = g;
+    if (plan) a.plan = plan->p;
+    a.q = {const_cast<void*>(d_q), q_tok, q_head, n_q_heads};
+    a.q_out = {d_q ? d_q_out : nullptr, qo_tok, qo_head, n_q_heads};
+    a.k = {const_cast<void*>(d_k), k_tok, k_head, g.n_kv_heads};
+    a.v = {const_cast<void*>(d_v), v_tok, v_head, g.n_kv_heads};
+    a.q_norm = d_q_norm_w;
+    a.k_norm = d_k_norm_w;
+    a.eps = eps;
+    a.tok_start = d_tok_start;
+    a.start_pos = d_start_pos;
+    a.page_table = d_page_table;
+    a.max_pages = max_pages;
+    a.n_seq = n_seq;
+    a.n_rows = n_rows;
+    a.dtype = dtype;
+    a.k_val = d_k_values;
+    a.v_val = d_v_values;
+    PI_HIP(h, pi::launch_q4_append(a, pick(h, stream)), "pi_q4_append");
+    return PI_OK;
+}
+
+namespace {
+int q4_records(pi_handle h, const char* what, bool write, pi_q4_pool pool, const int32_t* d_page_table, int32_t max_pages, int32_t seq,
+               int32_t start, int32_t n_tok, uint8_t* kc, uint16_t* ks, uint8_t* vc, uint16_t* vs, void* stream) {
+    PI_CHECK_HANDLE(h);
+    if (!pool || !d_page_table || (n_tok > 0 && (!kc || !ks || !vc || !vs))) return fail(h, PI_ERR_INVALID_ARG, "%s: null argument", what);
+    if (seq < 0 || start < 0 || n_tok < 0 || max_pages <= 0 || max_pages > (1 << 26))
+        return fail(h, PI_ERR_INVALID_ARG, "%s: seq=%d start=%d n_tok=%d max_pages=%d", what, seq, start, n_tok, max_pages);
+    if (pool->owner->device != h->device)
+        return fail(h, PI_ERR_INVALID_ARG, "%s: the pool is on device %d", what, pool->owner->device);
+    if (n_tok == 0) return PI_OK;
+    const DeviceScope on(h->device);
+    PI_HIP(h, on.err, what);
+    PI_HIP(h, pi::launch_q4_records(pool->g, write, d_page_table + (size_t)seq * max_pages, max_pages, start, n_tok, kc, ks, vc, vs,
+                                    pick(h, stream)),
+           what);
+    return PI_OK;
+}
+}  // namespace
+
+int pi_q4_read(pi_handle h, pi_q4_pool pool, const int32_t* d_page_table, int32_t max_pages, int32_t seq, int32_t start, int32_t n_tok,
+               uint8_t* d_k_codes, uint16_t* d_k_scales, uint8_t* d_v_codes, uint16_t* d_v_scales, void* stream) {
+    return q4_records(h, "pi_q4_read", false, pool, d_page_table, max_pages, seq, start, n_tok, d_k_codes, d_k_scales, d_v_codes,
+                      d_v_scales, stream);
+}
+
+int pi_q4_write(pi_handle h, pi_q4_pool pool, const int32_t* d_page_table, int32_t max_pages, int32_t seq, int32_t start, int32_t n_tok,
+                const uint8_t* d_k_codes, const uint16_t* d_k_scales, const uint8_t* d_v_codes, const uint16_t* d_v_scales,
+                void* stream) {
+    return q4_records(h, "pi_q4_write", true, pool, d_page_table, max_pages, seq, start, n_tok, const_cast<uint8_t*>(d_k_codes),
+                      const_cast<uint16_t*>(d_k_scales), const_cast<uint8_t*>(d_v_codes), const_cast<uint16_t*>(d_v_scales), stream);
+}
+
+namespace {
+// The checks of both attentions and their launch arguments; max_tok and tok_start are 1 and null for a decode.
+int q4_attn_args(pi_handle h, const char* what, pi_q4_pool pool, int32_t dtype, int32_t n_rows, int32_t n_seq, int32_t max_tok,
+                 int32_t max_pages, int32_t max_ctx, int32_t n_q_heads, int32_t gqa_mode, pi::Q4AttnArgs* a, pi::Q4Plan* plan) {
+    PI_CHECK_HANDLE(h);
+    if (!pool) return fail(h, PI_ERR_INVALID_ARG, "%s: null argument", what);
+    const pi::Q4Geom& g = pool->g;
+    if (dtype < PI_F32 || dtype > PI_BF16) return fail(h, PI_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+    if (n_rows < 0 || n_seq < 0 || n_seq > pi::kQ4MaxBatch || max_tok < 0 || max_pages <= 0 || max_pages > (1 << 26) || max_ctx < 0 ||
+        n_q_heads <= 0 || n_q_heads > 65536)
+        return fail(h, PI_ERR_INVALID_ARG, "%s: rows=%d sequences=%d (at most %d) max_tok=%d max_pages=%d max_ctx=%d n_q_heads=%d", what,
+                    n_rows, n_seq, pi::kQ4MaxBatch, max_tok, max_pages, max_ctx, n_q_heads);
+    if (gqa_mode != PI_GQA_MODULO && gqa_mode != PI_GQA_GROUPED) return fail(h, PI_ERR_INVALID_ARG, "%s: gqa_mode %d", what, gqa_mode);
+    if (gqa_mode == PI_GQA_GROUPED && n_q_heads % g.n_kv_heads != 0)
+        return fail(h, PI_ERR_INVALID_ARG, "%s: grouped head map with n_q_heads %d not a multiple of n_kv_heads %d", what, n_q_heads,
+                    g.n_kv_heads);
+    if (pool->owner->device != h->device)
+        return fail(h, PI_ERR_INVALID_ARG, "%s: the pool is on device %d", what, pool->owner->device);
+    a->g = g;
+    a->dtype = dtype;
+    a->max_pages = max_pages;
+    a->use_pages = max_ctx ? std::min(max_pages, (int32_t)(((int64_t)max_ctx + pi::kPageTokens - 1) / pi::kPageTokens)) : max_pages;
+    a->batch = n_seq;
+    a->n_rows = n_rows;
+    a->max_tok = std::min(max_tok, n_rows);
+    a->n_q_heads = n_q_heads;
+    a->gqa_mode = gqa_mode;
+    *plan = pi::q4_plan(*a, h->device);
+    if (!plan->grid) return fail(h, PI_ERR_UNSUPPORTED, "%s: more work items than 2^31", what);
+    return PI_OK;
+}
+
+int q4_attn(pi_handle h, const char* what, pi_q4_pool pool, const void* d_q, int32_t dtype, const int32_t* d_tok_start, int32_t n_rows,
+            const int32_t* d_pos, int32_t n_seq, int32_t max_tok, const int32_t* d_page_table, int32_t max_pages, int32_t max_ctx,
+            int32_t n_q_heads, int32_t gqa_mode, float scale, const void* d_gate, void* d_out, void* d_ws, size_t ws_bytes,
+            void* stream) {
+    pi::Q4AttnArgs a{};
+    pi::Q4Plan plan;
+    if (int rc = q4_attn_args(h, what, pool, dtype, n_rows, n_seq, max_tok, max_pages, max_ctx, n_q_heads, gqa_mode, &a, &plan)) return rc;
+    if (n_rows == 0 || n_seq == 0 || max_tok == 0) return PI_OK;  // empty tensors have no address
+    if (!d_q || !d_out || !d_pos || !d_page_table) return fail(h, PI_ERR_INVALID_ARG, "%s: null argument", what);
+    for (const void* p : {d_q, d_gate, static_cast<const void*>(d_out), static_cast<const void*>(d_ws)})
+        if (reinterpret_cast<uintptr_t>(p) % 16) return fail(h, PI_ERR_INVALID_ARG, "%s: q, gate, out and ws must be 16-byte aligned", what);
+    if (plan.ws_bytes && (!d_ws || ws_bytes < plan.ws_bytes))
+        return fail(h, PI_ERR_INVALID_ARG, "%s: the workspace holds %zu bytes, %zu are needed", what, d_ws ? ws_bytes : (size_t)0,
+                    plan.ws_bytes);
+    a.q = d_q;
+    a.gate = d_gate;
+    a.out = d_out;
+    a.page_table = d_page_table;
+    a.tok_start = d_tok_start;
+    a.pos = d_pos;
+    a.scale = scale;
+    const DeviceScope on(h->device);
+    PI_HIP(h, on.err, what);
+    PI_HIP(h, pi::launch_q4_attn(a, plan, d_ws, pick(h, stream)), what);
+    return PI_OK;
+}
+}  // namespace
+
+int pi_q4_attn_ws_bytes(pi_handle h, pi_q4_pool pool, int32_t dtype, int32_t n_rows, int32_t n_seq, int32_t max_tok, int32_t max_pages,
+                        int32_t max_ctx, int32_t n_q_heads, int32_t gqa_mode, size_t* bytes) {
+    PI_CHECK_HANDLE(h);
+    if (!bytes) return fail(h, PI_ERR_INVALID_ARG, "pi_q4_attn_ws_bytes: null argument");
+    *bytes = 0;
+    pi::Q4AttnArgs a{};
+    pi::Q4Plan plan;
+    if (int rc = q4_attn_args(h, "pi_q4_attn_ws_bytes", pool, dtype, n_rows, n_seq, max_tok, max_pages, max_ctx, n_q_heads, gqa_mode, &a,
+                              &plan))
+        return rc;
+    *bytes = plan.ws_bytes;
+    return PI_OK;
+}
+
+int pi_q4_attn_decode(pi_handle h, pi_q4_pool pool, const void* d_q, int32_t dtype, const int32_t* d_page_table, int32_t max_pages,
+                      int32_t max_ctx, const int32_t* d_ctx_len, int32_t batch, int32_t n_q_heads, int32_t gqa_mode, float scale,
+                      const void* d_gate, void* d_out, void* d_ws, size_t ws_bytes, void* stream) {
+    return q4_attn(h, "pi_q4_attn_decode", pool, d_q, dtype, nullptr, batch, d_ctx_len, batch, 1, d_page_table, max_pages, max_ctx,
+                   n_q_heads, gqa_mode, scale, d_gate, d_out, d_ws, ws_bytes, stream);
+}
+
+int pi_q4_attn_prefill(pi_handle h, pi_q4_pool pool, const void* d_q, int32_t dtype, int32_t n_rows, const int32_t* d_tok_start,
+                       const int32_t* d_start_pos, int32_t n_seq, int32_t max_tok, const int32_t* d_page_table, int32_t max_pages,
+                       int32_t max_ctx, int32_t n_q_heads, int32_t gqa_mode, float scale, const void* d_gate, void* d_out, void* d_ws,
+                       size_t ws_bytes, void* stream) {
+    PI_CHECK_HANDLE(h);
+    if (!d_tok_start && n_rows > 0) return fail(h, PI_ERR_INVALID_ARG, "pi_q4_attn_prefill: null argument");
+    return q4_attn(h, "pi_q4_attn_prefill", pool, d_q, dtype, d_tok_start, n_rows, d_start_pos, n_seq, max_tok, d_page_table, max_pages,
+                   max_ctx, n_q_heads, gqa_mode, scale, d_gate, d_out, d_ws, ws_bytes, stream);
 }
 
 }  // extern "C"

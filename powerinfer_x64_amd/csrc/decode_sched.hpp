@@ -59,9 +59,10 @@ struct Run {
 
 // The run starting at item `cur` of a workgroup whose range ends at `end`;
 // `b` is the sequence of the previous run (or find_seq's answer).  s_cum
-// holds the prefix sums of items_of(seq_tokens(.)) over the batch.
-PI_HD Run run_at(const int* s_cum, const int32_t* ctx_len, int max_pages, int n_kv,
-                 int item_pages, int b, int cur, int end) {
+// holds the prefix sums of items_of(len_of(.)) over the batch; len_of(b) is
+// sequence b's token count, at most 16 pages' worth per page-table column.
+template <typename Len>
+PI_HD Run run_of(const int* s_cum, const Len& len_of, int n_kv, int item_pages, int b, int cur, int end) {
     Run r;
     int nb = s_cum[b + 1] - s_cum[b];
     while (nb == 0 || cur >= n_kv * s_cum[b + 1]) {  // skip empty / finished sequences
@@ -72,12 +73,23 @@ PI_HD Run run_at(const int* s_cum, const int32_t* ctx_len, int max_pages, int n_
     r.kvh = (cur - n_kv * s_cum[b]) / nb;
     r.seg0 = n_kv * s_cum[b] + r.kvh * nb;
     r.run_end = imin(end, r.seg0 + nb);
-    r.len = seq_tokens(ctx_len[b], max_pages);
+    r.len = len_of(b);
     const int n_pages_b = (r.len + kPage - 1) / kPage;
     r.pg0 = (cur - r.seg0) * item_pages;
     r.pg1 = imin(n_pages_b, (r.run_end - r.seg0) * item_pages);
     r.whole = cur == r.seg0 && r.run_end == r.seg0 + nb;
     return r;
+}
+
+// run_of over context lengths clamped to the page-table row (seq_tokens).
+struct CtxLen {
+    const int32_t* ctx_len;
+    int max_pages;
+    PI_HD int operator()(int b) const { return seq_tokens(ctx_len[b], max_pages); }
+};
+PI_HD Run run_at(const int* s_cum, const int32_t* ctx_len, int max_pages, int n_kv,
+                 int item_pages, int b, int cur, int end) {
+    return run_of(s_cum, CtxLen{ctx_len, max_pages}, n_kv, item_pages, b, cur, end);
 }
 
 // Pages of wave `wave` in the sub-run starting at page `sub` of a run ending

@@ -1,0 +1,623 @@
+// q4_attn.hip -- attention over the 4-bit paged cache for few rows a KV head (gfx950): one token a sequence
+// (decode), or a short chunk.  Split over the keys, balanced over a ragged batch.
+//
+// Work: rows = (token, query head) of one KV head ride in the MFMA columns, 16 to a column block and
+// up to 4 blocks to a wavefront, so a K / V code is dequantised once for up to 64 rows.  Per pair of 16-token pages
+//   S^T[16 tok x 16 rows] = K[16 x D] . Q^T[D x 16]           (v_mfma_f32_16x16x32_f16, a page each)
+//   O^T[D x 16]          += V^T[D x 32 tok] . P^T[32 x 16]    (the same instruction, both pages at once)
+// A lane's scores are tokens 4 (lane / 16) + r of its column, and the V words are laid out so that exactly
+// these tokens are the lane's share of V^T (q4.hpp): P never crosses lanes.
+//
+// Rounding: K and V values are exact in f16, f16 / bf16 queries too (bf16 and f32 rows are first scaled by a power
+// of two, so that no exponent leaves f16).  P goes to f16 (2^-12 relative, below the rounding of a
+// 16-bit output).  f32 queries and their P are split into two f16 (22 bits) and multiplied twice.  The scale is
+// applied to the f32 scores.
+//
+// Bound: a long context by HBM (18 D bytes a page and KV head); the dequantisation costs about 1.5 VALU instructions
+// a code and runs beside the loads of the next pages.  A short one by launches and round trips.
+//
+// Schedule: decode_sched.hpp's items (pages of one (sequence, KV head, row block) segment), an equal contiguous range
+// to each of a persistent grid's workgroups; a segment inside one workgroup is written at once,
+// others leave (max, sum, O) for q4_merge_kernel.  Where every segment is one item the merge is not launched.
+#include "pi_device.hpp"
+#include "q4_launch.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace pi {
+namespace {
+
+constexpr int kWaves = sched::kWaves;
+constexpr int kThreads = 64 * kWaves;
+constexpr float kLazy = 8.0f;     // log2 headroom before the running max moves
+constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
+constexpr int kStage = 2048;      // floats a wavefront stages at a time for the merge in LDS
+constexpr long long kWholeBytes = 96 << 10;
+constexpr int kItemPages = 16;    // most pages of a work item
+
+// Words of consecutive lanes as one load each.
+template <int N> struct Words {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const char* p) {
+        if (N == 2) {
+            const u32x2 r = *reinterpret_cast<const u32x2*>(p);
+            w[0] = r[0];
+            w[1] = r[1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) {
+                const u32x4 r = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * i + e] = r[e];
+            }
+        }
+    }
+};
+template <> struct Words<1> {
+    uint32_t w[1];
+    __device__ __forceinline__ void load(const char* p) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
+};
+
+// A page of one KV head as a lane holds it.
+template <int D>
+struct Page {
+    static constexpr int NJ = D / kQ4Group;
+    Words<NJ> k, v;
+    Words<NJ / 2> ks;   // K scales of token lane % 16, group j in half j % 2 of word j / 2
+    Words<2 * NJ> vs;   // V scales of the lane's four tokens: (t0, t2), (t1, t3) of group j
+    __device__ __forceinline__ void load(const char* blk, int lane) {
+        k.load(blk + lane * (4 * NJ));
+        v.load(blk + 8 * D + lane * (4 * NJ));
+        ks.load(blk + 16 * D + (lane & 15) * (2 * NJ));
+        vs.load(blk + 17 * D + (lane >> 4) * (8 * NJ));
+    }
+};
+
+__device__ __forceinline__ int head_of(int kvh, int c, int n_kv, int group, int mode) {
+    return mode == 0 ? kvh + c * n_kv : kvh * group + c;
+}
+
+// Row r of a KV head's rows: token r / group, head r % group; the element offset of its first channel
+// in q / gate / out, or -1.
+__device__ __forceinline__ long long row_offset(const Q4AttnArgs& a, const Q4Rows& rw, int kvh, int r, int D) {
+    const int t = r / a.group, c = r - t * a.group;
+    if (t >= rw.n) return -1;
+    const int h = head_of(kvh, c, a.g.n_kv_heads, a.group, a.gqa_mode);
+    if (h >= a.n_q_heads) return -1;
+    return ((long long)(rw.first + t) * a.n_q_heads + h) * D;
+}
+
+__device__ __forceinline__ float sigmoidf_(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+__device__ __forceinline__ Q4Rows rows_of(const Q4AttnArgs& a, int b) {
+    Q4Rows r = q4_rows(a.tok_start, a.pos, b, a.n_rows, a.max_tok, a.use_pages);
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void load8f(const T* p, float* x) {
+    constexpr int W = 16 / sizeof(T);
+    typedef T tv __attribute__((ext_vector_type(W)));
+#pragma unroll
+    for (int j = 0; j < 8 / W; ++j) {
+        const tv r = *reinterpret_cast<const tv*>(p + W * j);
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[W * j + i] = to_f32(r[i]);
+    }
+}
+
+// Query operand of one 16-row block: channels 32 j + 8 grp + e of the lane's row, scaled by 2^-ex.
+template <typename T, int D>
+struct Query {
+    static constexpr int NJ = D / kQ4Group, PREC = std::is_same<T, float>::value ? 2 : 1;
+    f16x8 r[PREC][NJ];
+    // returns the factor from a raw product to log2 units
+    __device__ __forceinline__ float load(const T* q, long long off, int grp, float scale) {
+        float x[8 * NJ];
+        const T* p = q + (off < 0 ? 0 : off) + 8 * grp;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) load8f(p + 32 * j, x + 8 * j);
+        float f = 1.f, back = scale * kLog2e;
+        if (!std::is_same<T, f16>::value) {
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8 * NJ; ++i) mx = fmaxf(mx, fabsf(x[i]));
+            mx = wave_max_xor(mx, 16);
+            mx = wave_max_xor(mx, 32);
+            // the row's largest magnitude to [1, 2)
+            const int ex = (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255u) - 127;
+            const int e1 = mx > 0.f && ex > -127 && ex < 127 ? ex : 0;
+            f = __builtin_bit_cast(float, (uint32_t)(127 - e1) << 23);
+            back = ldexpf(back, e1);
+        }
+        if (off < 0) f = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = off < 0 ? 0.f : x[8 * j + e] * f;
+                const f16 h = to_f16(y);
+                r[0][j][e] = h;
+                if (PREC == 2) r[PREC - 1][j][e] = to_f16(y - (float)h);
+            }
+        return back;
+    }
+};
+
+template <int D, int NCB>
+struct Acc {
+    f32x4 o[NCB][D / 16];
+    float m[NCB], l[NCB];
+};
+
+// Two pages: scores, softmax, values.  lim[cb]: keys below it are seen by the lane's row; tok0[u]: first token
+// of page u; edge: some row's limit may fall inside (then tokens are compared).
+template <typename T, int D, int NCB>
+__device__ __forceinline__ void process(Acc<D, NCB>& acc, const Page<D>* pg, const Query<T, D>* q, const float* back, const int* lim,
+                                        const int* tok0, bool edge, int grp, const Q4Magic& mg) {
+    constexpr int NJ = D / kQ4Group, PREC = Query<T, D>::PREC;
+    f32x4 s[2][NCB];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) s[u][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const f16x2 sc = __builtin_bit_cast(f16x2, pg[u].ks.w[j / 2]);
+            const f16x8 kf = deq_k(pg[u].k.w[j], sc[j & 1], mg);
+#pragma unroll
+            for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+                for (int h = 0; h < PREC; ++h)
+                    s[u][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[cb].r[h][j], s[u][cb], 0, 0, 0);
+        }
+    }
+    f16x8 pb[NCB][PREC];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u][cb] *= back[cb];
+            if (edge) {
+                const int left = lim[cb] - tok0[u] - 4 * grp;  // tokens of the lane's four that count
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (r >= left) s[u][cb][r] = -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][cb][r]);
+        }
+        if (__any(mx > acc.m[cb] + kLazy)) {
+            mx = wave_max_xor(mx, 16);
+            mx = wave_max_xor(mx, 32);
+            const float m_new = fmaxf(acc.m[cb], mx);
+            const float alpha = fast_exp2(acc.m[cb] - m_new);
+            acc.l[cb] *= alpha;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) acc.o[cb][t] *= alpha;
+            acc.m[cb] = m_new;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            float p[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) p[r] = fast_exp2(s[u][cb][r] - acc.m[cb]);
+            sum += (p[0] + p[1]) + (p[2] + p[3]);
+            const float pv[4] = {p[0], p[2], p[1], p[3]};  // the order of the V codes
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const f16 h = to_f16(pv[r]);
+                pb[cb][0][4 * u + r] = h;
+                if (PREC == 2) pb[cb][PREC - 1][4 * u + r] = to_f16(pv[r] - (float)h);
+            }
+        }
+        acc.l[cb] += sum;
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const f16x2 a0 = __builtin_bit_cast(f16x2, pg[0].vs.w[2 * j]), b0 = __builtin_bit_cast(f16x2, pg[0].vs.w[2 * j + 1]);
+        const f16x2 a1 = __builtin_bit_cast(f16x2, pg[1].vs.w[2 * j]), b1 = __builtin_bit_cast(f16x2, pg[1].vs.w[2 * j + 1]);
+        const f16 off = (f16)-72.0f;
+        const f16x2 oa0 = a0 * off, ob0 = b0 * off, oa1 = a1 * off, ob1 = b1 * off;
+        const uint32_t w0 = pg[0].v.w[j], w1 = pg[1].v.w[j];
+        const f16x8 lo = join4(deq_pair(w0 << 4, a0, oa0, mg), deq_pair(w0 >> 4, b0, ob0, mg), deq_pair(w1 << 4, a1, oa1, mg),
+                               deq_pair(w1 >> 4, b1, ob1, mg));
+        const f16x8 hi = join4(deq_pair(w0, a0, oa0, mg), deq_pair(w0 >> 8, b0, ob0, mg), deq_pair(w1, a1, oa1, mg),
+                               deq_pair(w1 >> 8, b1, ob1, mg));
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb)
+#pragma unroll
+            for (int h = 0; h < PREC; ++h) {
+                acc.o[cb][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pb[cb][h], acc.o[cb][2 * j], 0, 0, 0);
+                acc.o[cb][2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pb[cb][h], acc.o[cb][2 * j + 1], 0, 0, 0);
+            }
+    }
+}
+
+struct Q4Ws {
+    float* o;       // [slot][cols][D]
+    float* ml;      // [slot][cols][2]
+    int32_t* runs;  // [segment][2]
+};
+
+// Prefix sums of the sequences' items into s_cum; returns their total.
+__device__ __forceinline__ int scan_items(const Q4AttnArgs& a, int* s_cum, int* s_red) {
+    const int tid = threadIdx.x;
+    int carry = 0;
+    for (int base = 0; base < a.batch; base += kThreads) {
+        const int b = base + tid;
+        const int n = b < a.batch ? sched::items_of(rows_of(a, b).len, a.item_pages) : 0;
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o, 64);
+            if ((tid & 63) >= o) x += y;
+        }
+        if ((tid & 63) == 63) s_red[tid >> 6] = x;
+        __syncthreads();
+        int wsum = 0;
+        for (int w = 0; w < (tid >> 6); ++w) wsum += s_red[w];
+        const int incl = carry + wsum + x;
+        if (b < a.batch) s_cum[b] = incl - n;
+        carry += s_red[0] + s_red[1] + s_red[2] + s_red[3];
+        __syncthreads();
+    }
+    if (tid == 0) s_cum[a.batch] = carry;
+    __syncthreads();
+    return carry;
+}
+
+struct LenOf {
+    const Q4AttnArgs& a;
+    __device__ __forceinline__ int operator()(int b) const { return rows_of(a, b).len; }
+};
+
+template <typename T, int D, int NCB>
+__global__ __launch_bounds__(kThreads) void q4_attn_kernel(Q4AttnArgs a, Q4Ws ws, int stage) {
+    extern __shared__ __attribute__((aligned(16))) float s_dyn[];  // [4][stage] staged O, then s_cum[batch + 1]
+    __shared__ int s_red[4];
+    __shared__ float s_m[kWaves][16 * NCB];
+    __shared__ float s_l[kWaves][16 * NCB];
+    float* s_o = s_dyn;
+    int* s_cum = reinterpret_cast<int*>(s_dyn + kWaves * stage);
+
+    const Q4Magic mg;
+    const int n_kv = a.g.n_kv_heads, n_seg = n_kv * a.n_cb, tid = threadIdx.x;
+    if (!ws.runs)  // no merge follows: the rows of sequences without keys are zeroed here
+        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+            const Q4Rows rw = rows_of(a, b);
+            if (rw.len != 0) continue;
+            T* out = static_cast<T*>(a.out) + (size_t)rw.first * a.n_q_heads * D;
+            for (size_t i = tid; i < (size_t)rw.n * a.n_q_heads * D; i += kThreads) out[i] = from_f32<T>(0.f);
+        }
+    const int n_items = n_seg * scan_items(a, s_cum, s_red);
+    const int chunk = (n_items + gridDim.x - 1) / gridDim.x;
+    int cur = blockIdx.x * chunk;
+    const int end = min(n_items, cur + chunk);
+    if (cur >= end) return;
+
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+    const size_t blk_bytes = q4_block_bytes(D);
+
+    int b = sched::find_seq(s_cum, a.batch, n_seg, cur);
+    while (cur < end) {
+        const sched::Run run = sched::run_of(s_cum, LenOf{a}, n_seg, a.item_pages, b, cur, end);
+        b = run.b;
+        const int sidx = run.kvh, kvh = sidx / a.n_cb, row0 = (sidx % a.n_cb) * a.cols;
+        const Q4Rows rw = rows_of(a, b);
+        const size_t seg = (size_t)b * n_seg + sidx;
+        if (cur == run.seg0 && tid == 0 && ws.runs) {
+            int wg1;
+            const int n_runs = sched::merge_runs(s_cum, n_seg, chunk, b, sidx, &wg1);
+            ws.runs[2 * seg] = wg1;
+            ws.runs[2 * seg + 1] = n_runs;
+        }
+        if (row0 >= rw.n * a.group) {  // a row block past the sequence's rows
+            cur = run.run_end;
+            continue;
+        }
+        const int first_lim = rw.start + row0 / a.group + 1;  // keys that every row of the block sees
+        Query<T, D> q[NCB];
+        Acc<D, NCB> acc;
+        float back[NCB];
+        int lim[NCB];
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+            const int r = cb * 16 + col;
+            const long long off = r < a.cols ? row_offset(a, rw, kvh, row0 + r, D) : -1;
+            back[cb] = q[cb].load(static_cast<const T*>(a.q), off, grp, a.scale);
+            lim[cb] = min(rw.start + (row0 + r) / a.group + 1, rw.len);
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) acc.o[cb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            acc.m[cb] = -1e30f;
+            acc.l[cb] = 0.f;
+        }
+        const int32_t* pt = a.page_table + (size_t)b * a.max_pages;
+        for (int sub = run.pg0; sub < run.pg1; sub += sched::kSubPages) {
+            int first, n_my;
+            sched::sub_pages(sub, run.pg1, wave, &first, &n_my);
+            // A page id outside the pool holds no tokens: page 0 is read in its place, all of it masked.
+            const int pid_raw = lane < n_my ? pt[first + kWaves * lane] : 0;
+            const bool bad = !sched::page_ok(pid_raw, a.g.n_pages);
+            const int pid_v = bad ? 0 : pid_raw;
+            const uint64_t bad_pages = __ballot(bad);
+            const int first_pid = __builtin_amdgcn_readfirstlane(pid_v);
+            auto load_pair = [&](Page<D>* dst, int i) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int j = 2 * i + u;
+                    const int pid = j < n_my ? __builtin_amdgcn_readlane(pid_v, j) : first_pid;
+                    dst[u].load(a.g.base + ((size_t)pid * n_kv + kvh) * blk_bytes, lane);
+                }
+            };
+            constexpr int kNone = 0x7fffffc0;  // a page whose tokens are past every limit
+            auto run_pair = [&](const Page<D>* pg, int i) {
+                int tok0[2];
+                bool edge = false;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int j = 2 * i + u;
+                    const int t = (first + kWaves * j) * sched::kPage;
+                    const bool on = j < n_my && !((bad_pages >> j) & 1);
+                    tok0[u] = on ? t : kNone;
+                    edge = edge || !on || t + sched::kPage > first_lim;
+                }
+                process<T, D, NCB>(acc, pg, q, back, lim, tok0, edge, grp, mg);
+            };
+            const int n_iter = (n_my + 1) / 2;
+            if (n_iter > 0) {
+                Page<D> now[2], next[2];
+                load_pair(now, 0);
+                for (int i = 0; i < n_iter - 1; ++i) {
+                    load_pair(next, i + 1);
+                    run_pair(now, i);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) now[u] = next[u];
+                }
+                run_pair(now, n_iter - 1);
+            }
+        }
+        // ---- the 4 wavefronts' shares meet in LDS, `stage` floats of rows at a time ----
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+            acc.l[cb] = wave_sum_xor(acc.l[cb], 16);
+            acc.l[cb] = wave_sum_xor(acc.l[cb], 32);
+            if (grp == 0) {
+                s_m[wave][16 * cb + col] = acc.m[cb];
+                s_l[wave][16 * cb + col] = acc.l[cb];
+            }
+        }
+        const size_t slot = (size_t)sched::run_slot(cur == run.seg0, b, sidx, n_seg, a.batch, blockIdx.x);
+        const int per = stage / D;  // rows staged at a time: a power of two up to 16
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+            for (int c0 = 0; c0 < 16; c0 += per) {
+                const int r0 = 16 * cb + c0;  // rows r0 .. r0 + per - 1 of the block
+                if (r0 >= a.cols) break;
+                if (col >= c0 && col < c0 + per) {
+#pragma unroll
+                    for (int t = 0; t < D / 16; ++t)
+                        *reinterpret_cast<f32x4*>(&s_o[wave * stage + (col - c0) * D + 16 * t + 4 * grp]) = acc.o[cb][t];
+                }
+                __syncthreads();
+                for (int idx = tid; idx < per * D; idx += kThreads) {
+                    const int c = idx / D, d = idx - c * D, r = r0 + c;
+                    if (r >= a.cols) break;
+                    float M = s_m[0][r];
+#pragma unroll
+                    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][r]);
+                    float o = 0.f, lsum = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) {
+                        const float f = fast_exp2(s_m[w][r] - M);
+                        o += f * s_o[w * stage + idx];
+                        lsum += f * s_l[w][r];
+                    }
+                    if (run.whole) {
+                        const long long off = row_offset(a, rw, kvh, row0 + r, D);
+                        if (off < 0) continue;
+                        float y = lsum == 0.f ? 0.f : o / lsum;  // every key masked: zeros (a NaN stays)
+                        if (a.gate) y *= sigmoidf_(to_f32(static_cast<const T*>(a.gate)[off + d]));
+                        static_cast<T*>(a.out)[off + d] = from_f32<T>(y);
+                    } else {
+                        ws.o[(slot * a.cols + r) * D + d] = o;
+                        if (d == 0) {
+                            ws.ml[(slot * a.cols + r) * 2] = M;
+                            ws.ml[(slot * a.cols + r) * 2 + 1] = lsum;
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+        }
+        cur = run.run_end;
+    }
+}
+
+// Joins the runs of the segments that span several workgroups' ranges and writes zeros for the rows of
+// sequences without keys.  A workgroup: 64 V values of one segment; its 4 wavefronts take every 4th run each.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void q4_merge_kernel(Q4AttnArgs a, Q4Ws ws, int D) {
+    typedef typename std::conditional<V == 4, f32x4, float>::type VT;
+    __shared__ float s_w[4][kMaxRuns];
+    __shared__ int s_slot[kMaxRuns];
+    __shared__ float s_inv[4];
+    __shared__ __attribute__((aligned(16))) VT s_acc[4][64];
+    const int sidx = blockIdx.y, b = blockIdx.z, n_seg = gridDim.y;
+    const int kvh = sidx / a.n_cb, row0 = (sidx % a.n_cb) * a.cols;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int cols = a.cols, GD = cols * D, e0 = blockIdx.x * 64 * V;
+    const size_t seg = (size_t)b * n_seg + sidx;
+    const Q4Rows rw = rows_of(a, b);
+    const int wg1 = ws.runs ? ws.runs[2 * seg] : 0, n_runs = ws.runs ? ws.runs[2 * seg + 1] : 0;
+    T* out = static_cast<T*>(a.out);
+    const int e = e0 + V * lane;
+    const int c = e / D, d = e - c * D;
+    const long long off = e < GD ? row_offset(a, rw, kvh, row0 + c, D) : -1;
+    if (rw.len == 0) {  // a softmax over nothing leaves zeros (and the run table was not written)
+        if (wave == 0 && off >= 0)
+            for (int i = 0; i < V; ++i) out[off + d + i] = from_f32<T>(0.f);
+        return;
+    }
+    if (row0 >= rw.n * a.group || n_runs <= 1) return;
+    for (int r = tid; r < n_runs; r += 256) s_slot[r] = (int)sched::run_slot(r == 0, b, sidx, n_seg, a.batch, wg1 + r - 1);
+    __syncthreads();
+    const int c_lo = e0 / D, c_hi = min(cols - 1, (e0 + 64 * V - 1) / D);
+    constexpr int kPre = 4;
+    const bool on = e < GD;
+    const float* po = ws.o + (on ? e : 0);
+    auto part = [&](int r) { return *reinterpret_cast<const VT*>(po + (size_t)s_slot[r] * GD); };
+    const VT zero = VT{};
+    VT pre[kPre];
+#pragma unroll
+    for (int j = 0; j < kPre; ++j) {
+        const int r = wave + 4 * j;
+        pre[j] = r < n_runs ? part(r) : zero;
+    }
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2* pml = reinterpret_cast<const f2*>(ws.ml);
+    if (wave <= c_hi - c_lo) {  // a wavefront a row of this block
+        const int cc = c_lo + wave;
+        const f2 ml0 = lane < n_runs ? pml[(size_t)s_slot[lane] * cols + cc] : f2{-1e30f, 0.f};
+        float M = ml0[0];
+        for (int r = lane + 64; r < n_runs; r += 64) M = fmaxf(M, pml[(size_t)s_slot[r] * cols + cc][0]);
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) M = wave_max_xor(M, m);
+        float lsum = 0.f;
+        if (lane < n_runs) {
+            const float w = fast_exp2(ml0[0] - M);
+            s_w[wave][lane] = w;
+            lsum = w * ml0[1];
+        }
+        for (int r = lane + 64; r < n_runs; r += 64) {
+            const f2 ml = pml[(size_t)s_slot[r] * cols + cc];
+            const float w = fast_exp2(ml[0] - M);
+            s_w[wave][r] = w;
+            lsum += w * ml[1];
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) lsum = wave_sum_xor(lsum, m);
+        if (lane == 0) s_inv[wave] = lsum == 0.f ? 0.f : 1.0f / lsum;
+    }
+    __syncthreads();
+    const int cw = (on ? c : c_lo) - c_lo;
+    const float* w = s_w[cw];
+    VT sum = zero;
+#pragma unroll
+    for (int j = 0; j < kPre; ++j) {
+        const int r = wave + 4 * j;
+        if (r < n_runs) sum += w[r] * pre[j];
+    }
+    for (int r = wave + 4 * kPre; r < n_runs; r += 4) sum += w[r] * part(r);
+    s_acc[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || off < 0) return;
+    VT res = ((s_acc[0][lane] + s_acc[1][lane]) + (s_acc[2][lane] + s_acc[3][lane])) * s_inv[cw];
+    const float* rp = reinterpret_cast<const float*>(&res);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float y = rp[i];
+        if (a.gate) y *= sigmoidf_(to_f32(static_cast<const T*>(a.gate)[off + d + i]));
+        out[off + d + i] = from_f32<T>(y);
+    }
+}
+
+template <typename T, int D, int NCB>
+int vgpr_wgs() {  // resident workgroups a CU by registers alone
+    static const int n = [] {
+        int v = 0;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, q4_attn_kernel<T, D, NCB>, kThreads, 0) != hipSuccess || v <= 0) v = 1;
+        return v;
+    }();
+    return n;
+}
+template <typename T>
+int wgs_of(int d, int ncb) {
+    if (d == 256) return ncb == 1 ? vgpr_wgs<T, 256, 1>() : vgpr_wgs<T, 256, 2>();
+    if (d == 128) return ncb == 1 ? vgpr_wgs<T, 128, 1>() : ncb == 2 ? vgpr_wgs<T, 128, 2>() : vgpr_wgs<T, 128, 4>();
+    return ncb == 1 ? vgpr_wgs<T, 64, 1>() : ncb == 2 ? vgpr_wgs<T, 64, 2>() : vgpr_wgs<T, 64, 4>();
+}
+
+int stage_floats(int cols, int d) {  // rows staged at a time: a power of two, at most 16
+    int per = std::min(16, kStage / d);
+    while (per > 1 && per / 2 >= cols) per /= 2;
+    return per * d;
+}
+
+template <typename T, int D, int NCB>
+hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStream_t s) {
+    Q4Ws ws{};
+    if (plan.merge) {
+        ws.o = static_cast<float*>(wsp);
+        ws.ml = ws.o + (size_t)plan.n_slots * a.cols * D;
+        ws.runs = reinterpret_cast<int32_t*>(ws.ml + (size_t)plan.n_slots * a.cols * 2);
+    }
+    const int stage = stage_floats(a.cols, D);
+    const size_t lds = (size_t)kWaves * stage * 4 + (size_t)(a.batch + 1) * 4;
+    hipLaunchKernelGGL((q4_attn_kernel<T, D, NCB>), dim3(plan.grid), dim3(kThreads), lds, s, a, ws, stage);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (plan.merge) {
+        const int n_seg = a.g.n_kv_heads * a.n_cb;
+        // 256 values a workgroup, or 64 where that leaves few workgroups
+        const long long wg4 = (long long)((a.cols * D + 255) / 256) * n_seg * a.batch;
+        if (wg4 >= 128)
+            hipLaunchKernelGGL((q4_merge_kernel<T, 4>), dim3((a.cols * D + 255) / 256, n_seg, a.batch), dim3(256), 0, s, a, ws, D);
+        else
+            hipLaunchKernelGGL((q4_merge_kernel<T, 1>), dim3((a.cols * D + 63) / 64, n_seg, a.batch), dim3(256), 0, s, a, ws, D);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_d(const Q4AttnArgs& a, const Q4Plan& p, void* ws, hipStream_t s) {
+    const int d = a.g.head_dim;
+    if (d == 256) return p.ncb == 1 ? launch_t<T, 256, 1>(a, p, ws, s) : launch_t<T, 256, 2>(a, p, ws, s);
+    if (d == 128)
+        return p.ncb == 1 ? launch_t<T, 128, 1>(a, p, ws, s) : p.ncb == 2 ? launch_t<T, 128, 2>(a, p, ws, s) : launch_t<T, 128, 4>(a, p, ws, s);
+    return p.ncb == 1 ? launch_t<T, 64, 1>(a, p, ws, s) : p.ncb == 2 ? launch_t<T, 64, 2>(a, p, ws, s) : launch_t<T, 64, 4>(a, p, ws, s);
+}
+
+}  // namespace
+
+Q4Plan q4_plan(Q4AttnArgs& a, int device) {
+    Q4Plan p{};
+    const int d = a.g.head_dim, n_kv = a.g.n_kv_heads;
+    a.group = a.gqa_mode == 0 ? (a.n_q_heads + n_kv - 1) / n_kv : a.n_q_heads / n_kv;
+    const long long rows = (long long)a.group * std::max(a.max_tok, 1);  // of a KV head, at most
+    const int most = d == 256 ? 2 : 4;
+    const long long blocks = (rows + 15) / 16;
+    p.ncb = blocks >= 3 ? most : (int)blocks;
+    p.ncb = p.ncb == 3 ? 4 : p.ncb;
+    a.n_cb = (int)((rows + 16 * p.ncb - 1) / (16 * p.ncb));
+    a.cols = (int)std::min<long long>(rows, 16 * p.ncb);
+    const int n_seg = n_kv * a.n_cb;
+    int cus = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0) cus = 256;
+    const int regs = a.dtype == 0 ? wgs_of<float>(d, p.ncb) : a.dtype == 1 ? wgs_of<f16>(d, p.ncb) : wgs_of<bf16>(d, p.ncb);
+    const size_t lds = (size_t)kWaves * stage_floats(a.cols, d) * 4 + (size_t)(a.batch + 1) * 4 + 1024;
+    const int per_cu = std::max(1, std::min<int>(regs, (int)((160 << 10) / lds)));
+    p.grid = std::min(cus * per_cu, kMaxRuns - 1);
+    // Items of 16 pages, halved while the launch's most items would not give every workgroup two.
+    const long long seg_pages = (long long)a.batch * n_seg * a.use_pages;
+    int ip = kItemPages;
+    while (ip > 1 && seg_pages / ip < 2LL * p.grid) ip >>= 1;
+    // A short segment is one item: read by one workgroup in less time than a merge's launch takes.
+    if ((long long)a.use_pages * q4_block_bytes(d) <= kWholeBytes) ip = std::max(ip, a.use_pages);
+    a.item_pages = ip;
+    p.merge = a.use_pages > ip;
+    p.n_slots = (long long)a.batch * n_seg + p.grid;
+    if ((long long)a.batch * n_seg * ((a.use_pages + ip - 1) / ip) > 0x7fffffffll || n_seg > 65535) p.grid = 0;  // the caller refuses
+    p.ws_bytes = p.merge ? ((size_t)p.n_slots * a.cols * (d + 2) + (size_t)2 * a.batch * n_seg) * 4 : 0;
+    return p;
+}
+
+hipError_t launch_q4_attn(const Q4AttnArgs& a, const Q4Plan& p, void* ws, hipStream_t s) {
+    return a.dtype == 0 ? launch_d<float>(a, p, ws, s) : a.dtype == 1 ? launch_d<f16>(a, p, ws, s) : launch_d<bf16>(a, p, ws, s);
+}
+
+}  // namespace pi

@@ -19,6 +19,8 @@ from . import _abi
 F32, F16, BF16 = 0, 1, 2
 MODULO, GROUPED = 0, 1
 PAGE_TOKENS = 16
+ROPE_LAYOUTS = {"pairs": 0, "halves": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 
 _DTYPE_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
@@ -668,3 +670,289 @@ def attn_prologue(dev: Device, q, k, v, pool: KvPool, page_table, start_pos, q_n
                                        _vp(page_table), page_table.shape[1], _vp(start_pos), n_seq,
                                        n_tok, hq, dev.stream()))
     return q, k
+
+
+# ---- rotary plans and the 4-bit cache ------------------------------------------------------
+
+
+def rope_freqs(rope_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+               orig_ctx: float = 4096, params: Optional[Sequence[float]] = None):
+    """Host only: (rope_dim / 2 rotary frequencies in float64, the factor of cos and sin).  `params`
+    are yarn's (fast, slow) turns, by default (32, 1), or bands' (low, high) turns, by default (1, 4)."""
+    if scaling not in ROPE_SCALINGS:
+        raise InvalidArg(f"scaling: {scaling!r} (one of {', '.join(ROPE_SCALINGS)})")
+    p = [] if scaling == "none" else [float(factor)]
+    if scaling in ("yarn", "bands"):
+        two = (32.0, 1.0) if scaling == "yarn" else (1.0, 4.0)
+        p += [float(orig_ctx), *(float(x) for x in (two if params is None else params))]
+    elif params is not None:
+        raise InvalidArg(f"params: scaling {scaling!r} takes none")
+    lib = _abi.load()
+    f = np.zeros(max(int(rope_dim) // 2, 1), np.float64)
+    m = ctypes.c_double()
+    rc = lib.pi_rope_scaled_freqs(int(rope_dim), float(base), ROPE_SCALINGS[scaling],
+                                  (ctypes.c_double * len(p))(*p) if p else None, len(p), f.ctypes.data,
+                                  ctypes.addressof(m))
+    if rc != 0:
+        raise _ERRORS.get(rc, PiError)(lib.pi_last_error(None).decode())
+    return f, m.value
+
+
+class RopePlan:
+    """Rotary frequencies on the device, for rope_apply and Q4Pool.append.  layout "halves" pairs channels
+    (i, i + rope_dim / 2), "pairs" (2i, 2i + 1); scaling and its arguments as rope_freqs, or the
+    frequencies themselves (`freqs`, rope_dim / 2 values, and `mscale`)."""
+
+    def __init__(self, dev: Device, rope_dim: int, base: float = 10000.0, layout: str = "halves",
+                 scaling: str = "none", factor: float = 1.0, orig_ctx: float = 4096,
+                 params: Optional[Sequence[float]] = None, freqs=None, mscale: Optional[float] = None):
+        self.p = None
+        self.dev, self.rope_dim, self.layout = dev, int(rope_dim), layout
+        if layout not in ROPE_LAYOUTS:
+            raise InvalidArg(f"layout: {layout!r} (one of {', '.join(ROPE_LAYOUTS)})")
+        if freqs is None:
+            f, m = rope_freqs(rope_dim, base, scaling, factor, orig_ctx, params)
+        else:
+            f, m = np.ascontiguousarray(freqs, np.float64).reshape(-1), 1.0
+            if f.size != self.rope_dim // 2:
+                raise InvalidArg(f"freqs: expected {self.rope_dim // 2} values, got {f.size}")
+        self.freqs, self.mscale = f, m if mscale is None else float(mscale)
+        p = ctypes.c_void_p()
+        dev.check(dev.lib.pi_rope_plan_create(dev.h, self.rope_dim, ROPE_LAYOUTS[layout], f.ctypes.data,
+                                              self.mscale, ctypes.byref(p)))
+        self.p = p
+
+    def close(self):
+        if self.p:
+            self.dev.lib.pi_rope_plan_destroy(self.p)
+            self.p = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _rows(t: torch.Tensor, name: str, dtype, shape, dev):
+    """A tensor of head rows [n, heads, D] at any strides of its first two dimensions: its address and them."""
+    if not isinstance(t, torch.Tensor):
+        raise InvalidArg(f"{name}: expected a torch.Tensor")
+    if t.device != dev:
+        raise InvalidArg(f"{name}: on {t.device}, expected {dev}")
+    if t.dtype != dtype:
+        raise InvalidArg(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if t.shape != shape:
+        raise InvalidArg(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    st, sh, sd = t.stride()
+    if sd != 1 and shape[2] > 1:
+        raise InvalidArg(f"{name}: the last dimension must be contiguous")
+    return t.data_ptr(), st, sh
+
+
+def _float_rows(t, name):
+    """The dtype code of a tensor of head rows."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        raise InvalidArg(f"{name}: expected a torch.Tensor [n, heads, D]")
+    code = _DTYPE_CODE.get(t.dtype)
+    if code is None:
+        raise Unsupported(f"{name}: dtype {t.dtype} (f32, f16 or bf16)")
+    return code
+
+
+def rope_apply(dev: Device, plan: RopePlan, q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor,
+               q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """q [n, Hq, D] and k [n, Hkv, D] (f32 / f16 / bf16, D contiguous, any other strides) rotated at
+    positions pos int32 [n], into q_out and k_out: new contiguous tensors by default, or q and k themselves for
+    a rotation in place.  Returns (q_out, k_out)."""
+    code, td = _float_rows(q, "q"), dev.torch_device
+    n, hq, d = q.shape
+    qp = _rows(q, "q", q.dtype, q.shape, td)
+    if q_out is None:
+        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=td)
+    qo = _rows(q_out, "q_out", q.dtype, q.shape, td)
+    kp = ko = (None, 0, 0)
+    hkv = 0
+    if k is not None:
+        _float_rows(k, "k")
+        hkv = k.shape[1]
+        kp = _rows(k, "k", q.dtype, (n, hkv, d), td)
+        if k_out is None:
+            k_out = torch.empty((n, hkv, d), dtype=q.dtype, device=td)
+        ko = _rows(k_out, "k_out", q.dtype, (n, hkv, d), td)
+    _need(pos, "pos", torch.int32, (n,), td)
+    dev.check(dev.lib.pi_rope_apply(dev.h, plan.p, code, n, d, pos.data_ptr(), *qp, hq, *qo, *kp, hkv, *ko,
+                                    dev.stream()))
+    return q_out, k_out
+
+
+class Q4Pool:
+    """Paged KV cache held in 4 bits (include/pi_attn.h): groups of 32 channels with an f16 scale, 4.5 bits
+    a value; 16-token pages addressed by the caller's page table, head_dim 64, 128 or 256."""
+
+    def __init__(self, dev: Device, n_pages: int, n_kv_heads: int, head_dim: int,
+                 page_tokens: int = PAGE_TOKENS):
+        self.p = None
+        self.dev = dev
+        self.n_pages, self.n_kv_heads, self.head_dim = n_pages, n_kv_heads, head_dim
+        p = ctypes.c_void_p()
+        dev.check(dev.lib.pi_q4_pool_create(dev.h, n_pages, page_tokens, n_kv_heads, head_dim,
+                                            ctypes.byref(p)))
+        self.p = p
+
+    @property
+    def nbytes(self) -> int:
+        return int(self.dev.lib.pi_q4_pool_bytes(self.p))
+
+    def close(self):
+        if self.p:
+            self.dev.lib.pi_q4_pool_destroy(self.p)
+            self.p = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, start_pos: torch.Tensor,
+               tok_start: Optional[torch.Tensor] = None, plan: Optional[RopePlan] = None,
+               q: Optional[torch.Tensor] = None, q_norm_w: Optional[torch.Tensor] = None,
+               k_norm_w: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               q_out: Optional[torch.Tensor] = None, values: bool = False):
+        """Appends k, v [n, Hkv, D] (f32 / f16 / bf16, D contiguous, any other strides): sequence s's rows
+        tok_start[s] .. tok_start[s + 1] - 1 (int32 [n_seq + 1]; None: one row a sequence) go to positions
+        start_pos[s] ... of page_table's row s, k normed by k_norm_w and rotated by plan on the way.  With q
+        [n, Hq, D], returns it normed and rotated (q_out: another tensor than q, a new one by default);
+        with `values`, (q_out, k, v) with the f16 [n, Hkv, D] values that the cache now holds (rows of no
+        sequence stay uninitialised)."""
+        d, td = self.dev, self.dev.torch_device
+        code = _float_rows(k, "k")
+        n, hkv, dh = k.shape
+        shape = (n, self.n_kv_heads, self.head_dim)
+        kp = _rows(k, "k", k.dtype, shape, td)
+        vp = _rows(v, "v", k.dtype, shape, td)
+        if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+            raise InvalidArg("page_table: expected a torch.Tensor [n_seq, max_pages]")
+        n_seq = start_pos.shape[0] if isinstance(start_pos, torch.Tensor) and start_pos.dim() == 1 else -1
+        _need(page_table, "page_table", torch.int32, dev=td)
+        _need(start_pos, "start_pos", torch.int32, (n_seq,), td)
+        if page_table.shape[0] < n_seq:
+            raise InvalidArg(f"page_table: shape {tuple(page_table.shape)}")
+        if tok_start is not None:
+            _need(tok_start, "tok_start", torch.int32, (n_seq + 1,), td)
+        qp = qo = (None, 0, 0)
+        hq = 0
+        if q is not None:
+            _float_rows(q, "q")
+            hq = q.shape[1]
+            qp = _rows(q, "q", k.dtype, (n, hq, dh), td)
+            if q_out is None:
+                q_out = torch.empty((n, hq, dh), dtype=q.dtype, device=td)
+            qo = _rows(q_out, "q_out", k.dtype, (n, hq, dh), td)
+        for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+            if w is not None:
+                _need(w, name, torch.float32, (dh,), td)
+        kv = torch.empty((2,) + shape, dtype=torch.float16, device=td) if values else None
+        at = kv.data_ptr() if values else None
+        d.check(d.lib.pi_q4_append(d.h, self.p, None if plan is None else plan.p, code, n, _vp(tok_start),
+                                   start_pos.data_ptr(), n_seq, page_table.data_ptr(), page_table.shape[1],
+                                   *qp, hq, *qo, *kp, *vp, _vp(q_norm_w), _vp(k_norm_w), float(eps), at,
+                                   at + kv[0].numel() * 2 if values else None, d.stream()))
+        return (q_out, kv[0], kv[1]) if values else q_out
+
+    def _record_shapes(self, n):
+        hk, d = self.n_kv_heads, self.head_dim
+        return ((torch.uint8, (n, hk, d // 2)), (torch.float16, (n, hk, d // 32))) * 2
+
+    def read(self, page_table: torch.Tensor, seq: int, start: int, n_tok: int):
+        """(k_codes, k_scales, v_codes, v_scales) of positions start .. start + n_tok - 1 of sequence seq:
+        uint8 [n_tok, Hkv, D / 2], even channel in the low bits, and f16 [n_tok, Hkv, D / 32]."""
+        d = self.dev
+        _need(page_table, "page_table", torch.int32, dev=d.torch_device)
+        if page_table.dim() != 2 or not 0 <= seq < page_table.shape[0]:
+            raise InvalidArg(f"seq {seq} of page_table {tuple(page_table.shape)}")
+        out = [torch.empty(s, dtype=t, device=d.torch_device) for t, s in self._record_shapes(max(int(n_tok), 0))]
+        d.check(d.lib.pi_q4_read(d.h, self.p, page_table.data_ptr(), page_table.shape[1], int(seq), int(start),
+                                 int(n_tok), *(t.data_ptr() for t in out), d.stream()))
+        return tuple(out)
+
+    def write(self, page_table: torch.Tensor, seq: int, start: int, k_codes: torch.Tensor,
+              k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor):
+        """Puts records that `read` gave back into the pages."""
+        d = self.dev
+        _need(page_table, "page_table", torch.int32, dev=d.torch_device)
+        if page_table.dim() != 2 or not 0 <= seq < page_table.shape[0]:
+            raise InvalidArg(f"seq {seq} of page_table {tuple(page_table.shape)}")
+        n = k_codes.shape[0] if isinstance(k_codes, torch.Tensor) and k_codes.dim() else 0
+        args = (k_codes, k_scales, v_codes, v_scales)
+        for name, t, (dt, shp) in zip(("k_codes", "k_scales", "v_codes", "v_scales"), args, self._record_shapes(n)):
+            _need(t, name, dt, shp, d.torch_device)
+        d.check(d.lib.pi_q4_write(d.h, self.p, page_table.data_ptr(), page_table.shape[1], int(seq), int(start), n,
+                                  *(t.data_ptr() for t in args), d.stream()))
+
+
+def _q4_attn(entry, dev, q, pool, page_table, n_seq, tok_start, pos, max_tok, max_ctx, gqa_mode, scale, gate, out,
+             ws):
+    code, td = _float_rows(q, "q"), dev.torch_device
+    _need(q, "q", dev=td)
+    n, hq, dh = q.shape
+    if dh != pool.head_dim:
+        raise InvalidArg(f"q head_dim {dh} != pool head_dim {pool.head_dim}")
+    _need(page_table, "page_table", torch.int32, dev=td)
+    if page_table.dim() != 2 or page_table.shape[0] < n_seq:
+        raise InvalidArg(f"page_table: shape {tuple(page_table.shape)}")
+    if gate is not None:
+        _need(gate, "gate", q.dtype, q.shape, td)
+    if out is None:
+        out = torch.empty_like(q)
+    _need(out, "out", q.dtype, q.shape, td)
+    max_pages, max_ctx = page_table.shape[1], 0 if max_ctx is None else int(max_ctx)
+    need = ctypes.c_size_t()
+    dev.check(dev.lib.pi_q4_attn_ws_bytes(dev.h, pool.p, code, n, n_seq, max_tok, max_pages, max_ctx, hq, gqa_mode,
+                                          ctypes.byref(need)))
+    if ws is None:  # torch's allocator keeps it with the stream, and with the graph under capture
+        ws = torch.empty(need.value, dtype=torch.uint8, device=td) if need.value else None
+    elif not isinstance(ws, torch.Tensor) or ws.device != td or not ws.is_contiguous():
+        raise InvalidArg("ws: expected a contiguous torch.Tensor on the device")
+    if scale is None:
+        scale = 1.0 / math.sqrt(dh)
+    ws_ptr, ws_bytes = (None, 0) if ws is None else (ws.data_ptr(), ws.numel() * ws.element_size())
+    if tok_start is None:
+        rc = entry(dev.h, pool.p, q.data_ptr(), code, page_table.data_ptr(), max_pages, max_ctx, pos.data_ptr(), n, hq,
+                   gqa_mode, float(scale), _vp(gate), out.data_ptr(), ws_ptr, ws_bytes, dev.stream())
+    else:
+        rc = entry(dev.h, pool.p, q.data_ptr(), code, n, tok_start.data_ptr(), pos.data_ptr(), n_seq, max_tok,
+                   page_table.data_ptr(), max_pages, max_ctx, hq, gqa_mode, float(scale), _vp(gate), out.data_ptr(),
+                   ws_ptr, ws_bytes, dev.stream())
+    dev.check(rc)
+    return out
+
+
+def q4_attn_decode(dev: Device, q: torch.Tensor, pool: Q4Pool, page_table: torch.Tensor, ctx_len: torch.Tensor,
+                   gqa_mode: int = MODULO, scale: Optional[float] = None, gate: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None,
+                   ws: Optional[torch.Tensor] = None):
+    """q [B, Hq, D] (f32 / f16 / bf16) -> out like q, over each sequence's ctx_len[b] tokens of the 4-bit cache.
+    max_ctx: a bound of ctx_len (default: the table's row).  ws: a workspace of the caller's; by default
+    the call takes one from torch's allocator."""
+    b = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else 0
+    _need(ctx_len, "ctx_len", torch.int32, (b,), dev.torch_device)
+    return _q4_attn(dev.lib.pi_q4_attn_decode, dev, q, pool, page_table, b, None, ctx_len, 1, max_ctx, gqa_mode, scale,
+                    gate, out, ws)
+
+
+def q4_attn_prefill(dev: Device, q: torch.Tensor, pool: Q4Pool, page_table: torch.Tensor, start_pos: torch.Tensor,
+                    tok_start: torch.Tensor, max_tok: Optional[int] = None, gqa_mode: int = MODULO,
+                    scale: Optional[float] = None, gate: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None,
+                    ws: Optional[torch.Tensor] = None):
+    """A chunk of tokens a sequence, causal: q [n, Hq, D], sequence s's rows tok_start[s] .. tok_start[s + 1] - 1
+    at positions start_pos[s] ... (their keys appended first) -> out like q.  max_tok: no sequence has more
+    rows (default: n).  Rows of no sequence are left as they were in `out`."""
+    n_seq = start_pos.shape[0] if isinstance(start_pos, torch.Tensor) and start_pos.dim() == 1 else -1
+    _need(start_pos, "start_pos", torch.int32, (n_seq,), dev.torch_device)
+    _need(tok_start, "tok_start", torch.int32, (n_seq + 1,), dev.torch_device)
+    n = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else 0
+    return _q4_attn(dev.lib.pi_q4_attn_prefill, dev, q, pool, page_table, n_seq, tok_start, start_pos,
+                    n if max_tok is None else int(max_tok), max_ctx, gqa_mode, scale, gate, out, ws)
