@@ -33,6 +33,7 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kLazy = 8.0f;     // log2 headroom before the running max moves
 constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
 constexpr int kStage = 2048;      // floats a wavefront stages at a time for the merge in LDS
+constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
 constexpr long long kWholeBytes = 96 << 10;
 constexpr int kItemPages = 16;    // most pages of a work item
 
@@ -589,6 +590,22 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     const int d = a.g.head_dim, n_kv = a.g.n_kv_heads;
     a.group = a.gqa_mode == 0 ? (a.n_q_heads + n_kv - 1) / n_kv : a.n_q_heads / n_kv;
     const long long rows = (long long)a.group * std::max(a.max_tok, 1);  // of a KV head, at most
+    int cus = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0) cus = 256;
+    if (rows > kTileRows) {
+        const int per = q4_tile_rows(d, a.dtype);
+        const long long n_blk = (rows + per - 1) / per, wgs = n_blk * n_kv * a.batch;
+        p.tiles = true;
+        // Few row blocks: their keys are split while that fills idle CUs and each part keeps 4 tiles.
+        long long splits = wgs >= cus ? 1 : std::min<long long>({8, cus / wgs, a.use_pages / 16});
+        splits = std::max<long long>(splits, 1);
+        p.splits = (int)splits;
+        p.n_blk = (int)n_blk;
+        p.grid = wgs * splits > 0x7fffffffll ? 0 : (int)(wgs * splits);  // 0: the caller refuses
+        p.merge = splits > 1;
+        p.ws_bytes = p.merge ? (size_t)splits * a.n_rows * a.n_q_heads * (d + 2) * 4 : 0;
+        return p;
+    }
     const int most = d == 256 ? 2 : 4;
     const long long blocks = (rows + 15) / 16;
     p.ncb = blocks >= 3 ? most : (int)blocks;
@@ -596,8 +613,6 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     a.n_cb = (int)((rows + 16 * p.ncb - 1) / (16 * p.ncb));
     a.cols = (int)std::min<long long>(rows, 16 * p.ncb);
     const int n_seg = n_kv * a.n_cb;
-    int cus = 0;
-    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || cus <= 0) cus = 256;
     const int regs = a.dtype == 0 ? wgs_of<float>(d, p.ncb) : a.dtype == 1 ? wgs_of<f16>(d, p.ncb) : wgs_of<bf16>(d, p.ncb);
     const size_t lds = (size_t)kWaves * stage_floats(a.cols, d) * 4 + (size_t)(a.batch + 1) * 4 + 1024;
     const int per_cu = std::max(1, std::min<int>(regs, (int)((160 << 10) / lds)));
@@ -617,6 +632,7 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
 }
 
 hipError_t launch_q4_attn(const Q4AttnArgs& a, const Q4Plan& p, void* ws, hipStream_t s) {
+    if (p.tiles) return launch_q4_tiles(a, p, ws, s);
     return a.dtype == 0 ? launch_d<float>(a, p, ws, s) : a.dtype == 1 ? launch_d<f16>(a, p, ws, s) : launch_d<bf16>(a, p, ws, s);
 }
 

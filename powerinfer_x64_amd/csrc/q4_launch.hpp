@@ -75,7 +75,8 @@ struct Q4AttnArgs {
 struct Q4Plan {
     bool tiles;          // the LDS-tiled kernel (many rows), else the column kernel
     int32_t grid, ncb;   // column kernel: workgroups, 16-row column blocks a segment
-    int32_t splits;      // tiled kernel: key splits
+    int32_t splits;      // tiled kernel: key splits of a row block,
+    int32_t n_blk;       // and row blocks of a sequence and KV head, at most
     bool merge;          // a second launch joins partials
     long long n_slots;
     size_t ws_bytes;
@@ -83,6 +84,8 @@ struct Q4Plan {
 // Fills a's planned fields.
 Q4Plan q4_plan(Q4AttnArgs& a, int device);
 hipError_t launch_q4_attn(const Q4AttnArgs& a, const Q4Plan& plan, void* ws, hipStream_t s);
+// Rows of a tiled workgroup.
+int q4_tile_rows(int head_dim, int dtype);
 hipError_t launch_q4_tiles(const Q4AttnArgs& a, const Q4Plan& plan, void* ws, hipStream_t s);
 
 }  // namespace pi

@@ -1,0 +1,518 @@
+// q4_prefill.hip -- attention of many rows a KV head over the 4-bit paged cache (gfx950): prompts and chunks.
+//
+// Work: the rows (token, query head) of one sequence and KV head, token by token, 32 to a wavefront. A workgroup walks
+// the keys its rows see in tiles of 64 (four pages); each tile's codes are dequantised once, into LDS, by all of its
+// wavefronts, so a code is unpacked once for 256 rows (128 where a wavefront needs a SIMD's registers alone).  Per tile and
+// wavefront, on v_mfma_f32_32x32x16_f16:
+//   S^T[64 x 32] = K . Q^T,   O^T[D x 32] += V^T . P^T
+// A lane owns one row's scores (half of them; lane + 32 has the rest), so a row's sum needs one cross-lane step at
+// the end, and its P values are the operand of the second product in place: the k index of a 16-key step is the order
+// in which a lane's scores and the dequantised V words come (q4.hpp).
+//
+// LDS: K tile [D / 8 chunks][64 keys] of 16 bytes, V tile [4 pages][2][D] of 16 bytes (8 keys of a channel), each doubled;
+// odd chunks / halves are shifted by 256 bytes so that a dequantising wavefront's stores and the operand reads both
+// cover all banks.
+//
+// Schedule (8 wavefronts, two a SIMD): in step t wavefronts 0..3 run the products (PV of tile t - 1, QK of tile t) and
+// then the softmax of tile t and the unpacking of K tile t + 1; wavefronts 4..7 run the softmax of tile t - 1 and the
+// unpacking of V tile t first and the products after: on each SIMD one wavefront's matrix instructions run beside the
+// other's vector instructions.  One barrier a step.
+//
+// Softmax: exps against the running max as it stands; only where a row's sum of a tile passes 2^13 (the first
+// tile, or a score outgrew the max) is the tile's max taken, O and l rescaled and the tile done again.
+//
+// f32 rows: q and P in two f16 parts (22 bits), each product twice, f32 accumulation.
+#include "pi_device.hpp"
+#include "q4_launch.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace pi {
+namespace {
+
+constexpr int kTile = 64;                    // keys
+constexpr int kTilePages = kTile / sched::kPage;
+constexpr float kRedo = 8192.0f;
+
+__device__ __forceinline__ float sigmoidf_(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+__device__ __forceinline__ void barrier_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int D> __device__ __forceinline__ int k_addr(int chunk, int key) { return (chunk * kTile + (key ^ (16 * (chunk & 1)))) * 16; }
+template <int D> __device__ __forceinline__ int v_addr(int page, int hh, int ch) { return ((page * 2 + hh) * D + (ch ^ (16 * hh))) * 16; }
+
+// One page's K codes of a lane (token lane % 16, chunks 4 j + lane / 16), or its V codes (tokens 4 (lane / 16) ..).
+template <int D>
+struct KPart {
+    static constexpr int NJ = D / kQ4Group;
+    uint32_t w[NJ];
+    f16 s[NJ];
+    __device__ __forceinline__ void load(const char* blk, int lane) {
+        __builtin_memcpy(w, __builtin_assume_aligned(blk + lane * (4 * NJ), 4 * NJ < 16 ? 4 * NJ : 16), 4 * NJ);
+        __builtin_memcpy(s, __builtin_assume_aligned(blk + 16 * D + (lane & 15) * (2 * NJ), 2 * NJ), 2 * NJ);
+    }
+    __device__ __forceinline__ void put(char* tile, int page, int lane, const Q4Magic& mg) const {
+        const int g = lane >> 4, key = page * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) *reinterpret_cast<f16x8*>(tile + k_addr<D>(4 * j + g, key)) = deq_k(w[j], s[j], mg);
+    }
+};
+template <int D>
+struct VPart {
+    static constexpr int NJ = D / kQ4Group;
+    uint32_t w[NJ];
+    f16x2 s[2 * NJ];
+    __device__ __forceinline__ void load(const char* blk, int lane) {
+        __builtin_memcpy(w, __builtin_assume_aligned(blk + 8 * D + lane * (4 * NJ), 4 * NJ < 16 ? 4 * NJ : 16), 4 * NJ);
+        __builtin_memcpy(s, __builtin_assume_aligned(blk + 17 * D + (lane >> 4) * (8 * NJ), 16), 8 * NJ);
+    }
+    __device__ __forceinline__ void put(char* tile, int page, int lane, const Q4Magic& mg) const {
+        const int q = lane >> 4, m = lane & 15;
+        const f16 off = (f16)-72.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const f16x2 a = s[2 * j], b = s[2 * j + 1], oa = a * off, ob = b * off;
+            const f16x2 l0 = deq_pair(w[j] << 4, a, oa, mg), l1 = deq_pair(w[j] >> 4, b, ob, mg);
+            const f16x2 h0 = deq_pair(w[j], a, oa, mg), h1 = deq_pair(w[j] >> 8, b, ob, mg);
+            char* p = tile + (q >> 1) * 8;
+            *reinterpret_cast<f16x4*>(p + v_addr<D>(page, q & 1, 32 * j + m)) = f16x4{l0[0], l0[1], l1[0], l1[1]};
+            *reinterpret_cast<f16x4*>(p + v_addr<D>(page, q & 1, 32 * j + 16 + m)) = f16x4{h0[0], h0[1], h1[0], h1[1]};
+        }
+    }
+};
+
+struct TileArgs {
+    float* o;   // partial O [split][row][D], row = packed token * n_q_heads + head
+    float* ml;  // partial (max, sum) [split][row][2]
+    int n_blk, splits;
+};
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, TileArgs ta) {
+    constexpr int KS = D / 16, NB = D / 32, PREC = std::is_same<T, float>::value ? 2 : 1;
+    constexpr int kRows = NW * 32, kBuf = kTile * D * 2;
+    extern __shared__ __attribute__((aligned(16))) char lds[];  // K tiles 0, 1, V tiles 0, 1
+    const int n_kv = a.g.n_kv_heads;
+    // KV heads fastest: with 8 of them each XCD's L2 sees one.  The last row blocks see most keys: first.
+    int id = blockIdx.x;
+    const int kvh = id % n_kv;
+    id /= n_kv;
+    const int split = id % ta.splits;
+    id /= ta.splits;
+    const int b = id % a.batch;
+    const int blk = ta.n_blk - 1 - id / a.batch;
+    const Q4Rows rw = q4_rows(a.tok_start, a.pos, b, a.n_rows, a.max_tok, a.use_pages);
+    const int row0 = blk * kRows, n_rows = rw.n * a.group;
+    if (row0 >= n_rows) return;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, hh = lane >> 5;
+    const Q4Magic mg;
+    // keys that the workgroup's last row sees, and its share of their tiles
+    const int last_tok = (min(row0 + kRows, n_rows) - 1) / a.group;
+    const int keys = (int)min((long long)rw.start + last_tok + 1, (long long)rw.len);
+    const int all_tiles = (keys + kTile - 1) / kTile;
+    const int t0 = (int)((long long)all_tiles * split / ta.splits), t1 = (int)((long long)all_tiles * (split + 1) / ta.splits);
+
+    // the lane's row
+    const int r = row0 + wave * 32 + col, tok = r / a.group, c = r - tok * a.group;
+    const int head = a.gqa_mode == 0 ? kvh + c * n_kv : kvh * a.group + c;
+    const bool on = tok < rw.n && head < a.n_q_heads;
+    const size_t row = on ? (size_t)(rw.first + tok) * a.n_q_heads + head : 0;
+    const int lim = on ? (int)min((long long)rw.start + tok + 1, (long long)rw.len) : 0;
+    // the wavefront's: keys that all rows see, and that any sees
+    const int w_tok0 = (row0 + wave * 32) / a.group, w_tok1 = (row0 + wave * 32 + 31) / a.group;
+    const int lim_all = (int)min((long long)rw.start + w_tok0 + 1, (long long)rw.len);
+    const int lim_any = w_tok0 < rw.n ? (int)min((long long)rw.start + min(w_tok1, rw.n - 1) + 1, (long long)rw.len) : 0;
+
+    // Q^T operand: channels 16 ks + 8 hh + e of the row
+    f16x8 q[PREC][KS];
+    float back = a.scale * kLog2e;
+    {
+        const T* p = static_cast<const T*>(a.q) + row * D + 8 * hh;
+        float x[8 * KS];
+        constexpr int W = 16 / sizeof(T);
+        typedef T tv __attribute__((ext_vector_type(W)));
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int j = 0; j < 8 / W; ++j) {
+                const tv v = *reinterpret_cast<const tv*>(p + 16 * k + W * j);
+#pragma unroll
+                for (int i = 0; i < W; ++i) x[8 * k + W * j + i] = on ? to_f32(v[i]) : 0.f;
+            }
+        float f = 1.f;
+        if (!std::is_same<T, f16>::value) {  // the row's largest magnitude to [1, 2)
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8 * KS; ++i) mx = fmaxf(mx, fabsf(x[i]));
+            mx = wave_max_xor(mx, 32);
+            const int ex = (int)((__builtin_bit_cast(uint32_t, mx) >> 23) & 255u) - 127;
+            const int e1 = mx > 0.f && ex > -127 && ex < 127 ? ex : 0;
+            f = __builtin_bit_cast(float, (uint32_t)(127 - e1) << 23);
+            back = ldexpf(back, e1);
+        }
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = x[8 * k + e] * f;
+                const f16 h = to_f16(y);
+                q[0][k][e] = h;
+                if (PREC == 2) q[PREC - 1][k][e] = to_f16(y - (float)h);
+            }
+    }
+    if (fabsf(back) < 1e-30f) back = copysignf(1e-30f, back);  // a scale of 0: all scores as good as equal, masks stay -inf
+    f32x16 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    float m = -1e30f, l = 0.f;
+    f32x16 s[2];
+    f16x8 pf[PREC][4];  // P of the tile's four 16-key steps
+
+    const int32_t* pt = a.page_table + (size_t)b * a.max_pages;
+    const int seq_pages = (rw.len + sched::kPage - 1) / sched::kPage;
+    // page ids of a tile in lanes 0..3 (a page past the sequence: none)
+    auto ids_of = [&](int t) {
+        const int p = t * kTilePages + (lane & 3);
+        return p < seq_pages ? pt[p] : -1;
+    };
+    auto bad_of = [&](int ids) { return (uint32_t)(__ballot(!sched::page_ok(ids, a.g.n_pages)) & 15u); };
+    auto block_of = [&](int ids, int page) {
+        const int id1 = __builtin_amdgcn_readlane(ids, page);
+        const int pid = sched::page_ok(id1, a.g.n_pages) ? id1 : 0;
+        return a.g.base + ((size_t)pid * n_kv + kvh) * q4_block_bytes(D);
+    };
+
+    // Both products read their LDS operands kAhead ahead and in this order (left alone, the compiler requests
+    // them all first and spills).
+    constexpr int kAhead = 4;
+    auto qk = [&](int t) {
+        const char* tile = lds + (t & 1) * kBuf;
+        auto frag = [&](int i) { return *reinterpret_cast<const f16x8*>(tile + k_addr<D>(2 * (i >> 1) + hh, 32 * (i & 1) + col)); };
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+        f16x8 f[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f[i] = frag(i);
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) {
+#pragma unroll
+            for (int h = 0; h < PREC; ++h)
+                s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % kAhead], q[h][i >> 1], s[i & 1], 0, 0, 0);
+            if (i + kAhead < 2 * KS) f[i % kAhead] = frag(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto pv = [&](int t) {
+        const char* tile = lds + (2 + (t & 1)) * kBuf;
+        auto frag = [&](int i) { return *reinterpret_cast<const f16x8*>(tile + v_addr<D>(i / NB, hh, 32 * (i % NB) + col)); };
+        f16x8 f[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f[i] = frag(i);
+#pragma unroll
+        for (int i = 0; i < 4 * NB; ++i) {
+#pragma unroll
+            for (int h = 0; h < PREC; ++h)
+                o[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % kAhead], pf[h][i / NB], o[i % NB], 0, 0, 0);
+            if (i + kAhead < 4 * NB) f[i % kAhead] = frag(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // P of the tile against m, its sum over the lane's 32 keys.
+    auto exps = [&] {
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float p = fast_exp2(fmaf(s[kb][8 * u + i], back, -m));
+                    sum += p;
+                    const int at = (i & 4) | ((i & 1) << 1) | ((i >> 1) & 1);  // 0, 2, 1, 3 of each four
+                    const f16 h = to_f16(p);
+                    pf[0][2 * kb + u][at] = h;
+                    if (PREC == 2) pf[PREC - 1][2 * kb + u][at] = to_f16(p - (float)h);
+                }
+        return sum;
+    };
+    auto softmax = [&](int t, uint32_t bad) {
+        if (bad != 0 || (t + 1) * kTile > lim_all) {  // scores that do not count: -inf after the factor, which is not 0
+            const int left = lim - t * kTile - 4 * hh;
+            const float none = back < 0.f ? INFINITY : -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (32 * kb + 8 * (e >> 2) + (e & 3) >= left || ((bad >> (2 * kb + (e >> 3))) & 1)) s[kb][e] = none;
+        }
+        float sum = exps();
+        while (__any(sum > kRedo)) {  // at most once: no P is above 1 after it
+            float mx = -1e30f;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e] * back);
+            mx = wave_max_xor(mx, 32);
+            const float m_new = fmaxf(m, mx), alpha = fast_exp2(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) o[i] *= alpha;
+            m = m_new;
+            sum = exps();
+        }
+        l += sum;
+    };
+
+    auto finish = [&] {
+        l = wave_sum_xor(l, 32);
+        if (!on) return;
+        // O^T: channel 32 nb + 8 (e / 4) + 4 hh + e % 4 of the lane's row
+        if (ta.splits > 1) {
+            const size_t prow = (size_t)split * a.n_rows * a.n_q_heads + row;
+            float* po = ta.o + prow * D + 4 * hh;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4*>(po + 32 * nb + 8 * i) =
+                        f32x4{o[nb][4 * i], o[nb][4 * i + 1], o[nb][4 * i + 2], o[nb][4 * i + 3]};
+            if (hh == 0) {
+                ta.ml[2 * prow] = m;
+                ta.ml[2 * prow + 1] = l;
+            }
+            return;
+        }
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        T* out = static_cast<T*>(a.out) + row * D + 4 * hh;
+        const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * D + 4 * hh : nullptr;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                t4 y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float v = o[nb][4 * i + e] * inv;
+                    if (gate) v *= sigmoidf_(to_f32(gate[32 * nb + 8 * i + e]));
+                    y[e] = from_f32<T>(v);
+                }
+                *reinterpret_cast<t4*>(out + 32 * nb + 8 * i) = y;
+            }
+    };
+
+    if (t0 >= t1) {
+        finish();
+        return;
+    }
+    // The wavefront's own last tile: its rows see none of the later ones, it only unpacks them.
+    const int n = max(t0, min(t1, (lim_any + kTile - 1) / kTile));
+    // ids of tiles t + 1 and t + 2 and the unusable pages of tile t, one step at a time
+    int i1 = ids_of(t0), i2 = ids_of(t0 + 1);
+    uint32_t bad = 0;
+    auto step_ids = [&](int t) {  // to step t
+        bad = bad_of(i1);
+        i1 = i2;
+        i2 = ids_of(t + 2);
+    };
+    if constexpr (NW == 8) {
+        const int page = wave & 3;
+        if (wave < 4) {
+            KPart<D> kp;
+            kp.load(block_of(i1, page), lane);
+            kp.put(lds + (t0 & 1) * kBuf, page, lane, mg);
+            kp.load(block_of(i2, page), lane);
+            barrier_lds();
+            auto unpack = [&](int t) {
+                if (t + 1 < t1) {
+                    kp.put(lds + ((t + 1) & 1) * kBuf, page, lane, mg);
+                    kp.load(block_of(i2, page), lane);
+                }
+                barrier_lds();
+            };
+            step_ids(t0);
+            if (n > t0) {
+                qk(t0);
+                softmax(t0, bad);
+            }
+            unpack(t0);
+            for (int t = t0 + 1; t < n; ++t) {
+                step_ids(t);
+                __builtin_amdgcn_s_setprio(2);
+                pv(t - 1);
+                qk(t);
+                __builtin_amdgcn_s_setprio(0);
+                softmax(t, bad);
+                unpack(t);
+            }
+            if (n > t0) pv(n - 1);
+            for (int t = max(n, t0 + 1); t <= t1; ++t) {
+                step_ids(t);
+                unpack(t);
+            }
+            finish();
+        } else {
+            VPart<D> vp;
+            vp.load(block_of(i1, page), lane);
+            barrier_lds();
+            auto unpack = [&](int t) {
+                if (t < t1) {
+                    vp.put(lds + (2 + (t & 1)) * kBuf, page, lane, mg);
+                    vp.load(block_of(i1, page), lane);
+                }
+            };
+            step_ids(t0);
+            unpack(t0);
+            if (n > t0) qk(t0);
+            barrier_lds();
+            uint32_t was = bad;
+            for (int t = t0 + 1; t < n; ++t) {
+                step_ids(t);
+                unpack(t);
+                softmax(t - 1, was);
+                was = bad;
+                __builtin_amdgcn_s_setprio(2);
+                pv(t - 1);
+                qk(t);
+                __builtin_amdgcn_s_setprio(0);
+                barrier_lds();
+            }
+            int t = t0 + 1;
+            if (n > t0) {
+                step_ids(n);
+                unpack(n);
+                softmax(n - 1, was);
+                pv(n - 1);
+                barrier_lds();
+                t = n + 1;
+            }
+            for (; t <= t1; ++t) {
+                step_ids(t);
+                unpack(t);
+                barrier_lds();
+            }
+            finish();
+        }
+    } else {
+        KPart<D> kp;
+        VPart<D> vp;
+        kp.load(block_of(i1, wave), lane);
+        vp.load(block_of(i1, wave), lane);
+        for (int t = t0; t < t1; ++t) {
+            step_ids(t);
+            // the other halves of the buffers may still be read in step t - 1, these by no wavefront
+            kp.put(lds + (t & 1) * kBuf, wave, lane, mg);
+            vp.put(lds + (2 + (t & 1)) * kBuf, wave, lane, mg);
+            barrier_lds();
+            kp.load(block_of(i1, wave), lane);
+            vp.load(block_of(i1, wave), lane);
+            if (t < n) {
+                qk(t);
+                softmax(t, bad);
+                pv(t);
+            }
+        }
+        finish();
+    }
+}
+
+// Joins the splits of each row: D / 4 threads a row.
+template <typename T>
+__global__ __launch_bounds__(256) void q4_tile_merge_kernel(Q4AttnArgs a, TileArgs ta, int D) {
+    const int per = 256 / (D / 4), rl = threadIdx.x / (D / 4), d = 4 * (threadIdx.x - rl * (D / 4));
+    const size_t rows = (size_t)a.n_rows * a.n_q_heads;
+    const size_t row = (size_t)blockIdx.x * per + rl;
+    if (row >= rows) return;
+    // rows of no sequence, and rows past max_tok, hold no partials
+    const int tok = (int)(row / a.n_q_heads);
+    bool mine = false;
+    for (int b0 = 0; b0 < a.batch; ++b0) {
+        const Q4Rows rw = q4_rows(a.tok_start, a.pos, b0, a.n_rows, a.max_tok, a.use_pages);
+        if (tok >= rw.first && tok < rw.first + rw.n) {
+            mine = true;
+            break;
+        }
+    }
+    if (!mine) return;
+    float mx = -1e30f, l = 0.f;
+    float mm[8], ll[8];
+    f32x4 oo[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        if (s >= ta.splits) break;
+        const size_t p = s * rows + row;
+        mm[s] = ta.ml[2 * p];
+        ll[s] = ta.ml[2 * p + 1];
+        oo[s] = *reinterpret_cast<const f32x4*>(ta.o + p * D + d);
+        mx = fmaxf(mx, mm[s]);
+    }
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        if (s >= ta.splits) break;
+        const float w = fast_exp2(mm[s] - mx);
+        o += w * oo[s];
+        l += w * ll[s];
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    t4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float v = o[e] * inv;
+        if (a.gate) v *= sigmoidf_(to_f32(static_cast<const T*>(a.gate)[row * D + d + e]));
+        y[e] = from_f32<T>(v);
+    }
+    *reinterpret_cast<t4*>(static_cast<T*>(a.out) + row * D + d) = y;
+}
+
+template <typename T, int D, int NW>
+hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& p, const TileArgs& ta, hipStream_t s) {
+    const size_t lds = (size_t)4 * kTile * D * 2;
+    if (lds > (64 << 10)) {
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_tile_kernel<T, D, NW>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL((q4_tile_kernel<T, D, NW>), dim3((unsigned)p.grid), dim3(NW * 64), lds, s, a, ta);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || ta.splits == 1) return e;
+    const int per = 256 / (D / 4);
+    const size_t rows = (size_t)a.n_rows * a.n_q_heads;
+    hipLaunchKernelGGL((q4_tile_merge_kernel<T>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s, a, ta, D);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_d(const Q4AttnArgs& a, const Q4Plan& p, const TileArgs& ta, hipStream_t s) {
+    constexpr int kWide = sizeof(T) == 2 ? 8 : 4;
+    switch (a.g.head_dim) {
+        case 64: return launch_t<T, 64, 8>(a, p, ta, s);
+        case 128: return launch_t<T, 128, kWide>(a, p, ta, s);
+        default: return launch_t<T, 256, 4>(a, p, ta, s);
+    }
+}
+
+}  // namespace
+
+int q4_tile_rows(int head_dim, int dtype) { return head_dim == 64 || (head_dim == 128 && dtype != 0) ? 256 : 128; }
+
+hipError_t launch_q4_tiles(const Q4AttnArgs& a, const Q4Plan& p, void* ws, hipStream_t s) {
+    TileArgs ta{};
+    ta.n_blk = p.n_blk;
+    ta.splits = p.splits;
+    if (p.splits > 1) {
+        ta.o = static_cast<float*>(ws);
+        ta.ml = ta.o + (size_t)p.splits * a.n_rows * a.n_q_heads * a.g.head_dim;
+    }
+    return a.dtype == 0 ? launch_d<float>(a, p, ta, s) : a.dtype == 1 ? launch_d<f16>(a, p, ta, s) : launch_d<bf16>(a, p, ta, s);
+}
+
+}  // namespace pi
