@@ -110,6 +110,29 @@ __device__ __forceinline__ f16x8 deq_k(uint32_t w, f16 s, const Q4Magic& mg) {
                  deq_pair(w >> 8, s2, off, mg));
 }
 
+// N words of a lane by its widest loads.
+template <int N> struct Words {
+    uint32_t w[N];
+    __device__ __forceinline__ void load(const char* p) {
+        if (N == 2) {
+            const u32x2 r = *reinterpret_cast<const u32x2*>(p);
+            w[0] = r[0];
+            w[1] = r[1];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i) {
+                const u32x4 r = reinterpret_cast<const u32x4*>(p)[i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * i + e] = r[e];
+            }
+        }
+    }
+};
+template <> struct Words<1> {
+    uint32_t w[1];
+    __device__ __forceinline__ void load(const char* p) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
+};
+
 // Scale words: an exact f16 on the format's grid whatever the bits were (records come from callers).
 __device__ __forceinline__ uint16_t q4_clean_scale(uint16_t bits) {
     const uint16_t mag = bits & 0x7ff0u, sign = bits & 0x8000u;

@@ -37,29 +37,6 @@ constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kern
 constexpr long long kWholeBytes = 96 << 10;
 constexpr int kItemPages = 16;    // most pages of a work item
 
-// Words of consecutive lanes as one load each.
-template <int N> struct Words {
-    uint32_t w[N];
-    __device__ __forceinline__ void load(const char* p) {
-        if (N == 2) {
-            const u32x2 r = *reinterpret_cast<const u32x2*>(p);
-            w[0] = r[0];
-            w[1] = r[1];
-        } else {
-#pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const u32x4 r = reinterpret_cast<const u32x4*>(p)[i];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[4 * i + e] = r[e];
-            }
-        }
-    }
-};
-template <> struct Words<1> {
-    uint32_t w[1];
-    __device__ __forceinline__ void load(const char* p) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
-};
-
 // A page of one KV head as a lane holds it.
 template <int D>
 struct Page {

@@ -46,35 +46,38 @@ template <int D> __device__ __forceinline__ int v_addr(int page, int hh, int ch)
 template <int D>
 struct KPart {
     static constexpr int NJ = D / kQ4Group;
-    uint32_t w[NJ];
-    f16 s[NJ];
+    Words<NJ> w;
+    Words<NJ / 2> s;
     __device__ __forceinline__ void load(const char* blk, int lane) {
-        __builtin_memcpy(w, __builtin_assume_aligned(blk + lane * (4 * NJ), 4 * NJ < 16 ? 4 * NJ : 16), 4 * NJ);
-        __builtin_memcpy(s, __builtin_assume_aligned(blk + 16 * D + (lane & 15) * (2 * NJ), 2 * NJ), 2 * NJ);
+        w.load(blk + lane * (4 * NJ));
+        s.load(blk + 16 * D + (lane & 15) * (2 * NJ));
     }
     __device__ __forceinline__ void put(char* tile, int page, int lane, const Q4Magic& mg) const {
         const int g = lane >> 4, key = page * 16 + (lane & 15);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) *reinterpret_cast<f16x8*>(tile + k_addr<D>(4 * j + g, key)) = deq_k(w[j], s[j], mg);
+        for (int j = 0; j < NJ; ++j)
+            *reinterpret_cast<f16x8*>(tile + k_addr<D>(4 * j + g, key)) = deq_k(w.w[j], __builtin_bit_cast(f16x2, s.w[j / 2])[j & 1], mg);
     }
 };
 template <int D>
 struct VPart {
     static constexpr int NJ = D / kQ4Group;
-    uint32_t w[NJ];
-    f16x2 s[2 * NJ];
+    Words<NJ> w;
+    Words<2 * NJ> s;
     __device__ __forceinline__ void load(const char* blk, int lane) {
-        __builtin_memcpy(w, __builtin_assume_aligned(blk + 8 * D + lane * (4 * NJ), 4 * NJ < 16 ? 4 * NJ : 16), 4 * NJ);
-        __builtin_memcpy(s, __builtin_assume_aligned(blk + 17 * D + (lane >> 4) * (8 * NJ), 16), 8 * NJ);
+        w.load(blk + 8 * D + lane * (4 * NJ));
+        s.load(blk + 17 * D + (lane >> 4) * (8 * NJ));
     }
     __device__ __forceinline__ void put(char* tile, int page, int lane, const Q4Magic& mg) const {
         const int q = lane >> 4, m = lane & 15;
         const f16 off = (f16)-72.0f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const f16x2 a = s[2 * j], b = s[2 * j + 1], oa = a * off, ob = b * off;
-            const f16x2 l0 = deq_pair(w[j] << 4, a, oa, mg), l1 = deq_pair(w[j] >> 4, b, ob, mg);
-            const f16x2 h0 = deq_pair(w[j], a, oa, mg), h1 = deq_pair(w[j] >> 8, b, ob, mg);
+            const f16x2 a = __builtin_bit_cast(f16x2, s.w[2 * j]), b = __builtin_bit_cast(f16x2, s.w[2 * j + 1]);
+            const f16x2 oa = a * off, ob = b * off;
+            const uint32_t x = w.w[j];
+            const f16x2 l0 = deq_pair(x << 4, a, oa, mg), l1 = deq_pair(x >> 4, b, ob, mg);
+            const f16x2 h0 = deq_pair(x, a, oa, mg), h1 = deq_pair(x >> 8, b, ob, mg);
             char* p = tile + (q >> 1) * 8;
             *reinterpret_cast<f16x4*>(p + v_addr<D>(page, q & 1, 32 * j + m)) = f16x4{l0[0], l0[1], l1[0], l1[1]};
             *reinterpret_cast<f16x4*>(p + v_addr<D>(page, q & 1, 32 * j + 16 + m)) = f16x4{h0[0], h0[1], h1[0], h1[1]};
@@ -187,60 +190,73 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
         return a.g.base + ((size_t)pid * n_kv + kvh) * q4_block_bytes(D);
     };
 
-    // Both products read their LDS operands kAhead ahead and in this order (left alone, the compiler requests
-    // them all first and spills).
+    // Both products read their LDS operands kAhead ahead, one read beside each matrix instruction (left alone, the
+    // compiler requests them all first and spills).
     constexpr int kAhead = 4;
+    auto paced = [](int n) {
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+            if (i < n - kAhead) {
+                __builtin_amdgcn_sched_group_barrier(0x008, PREC, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+        __builtin_amdgcn_sched_group_barrier(0x008, kAhead * PREC, 0);
+    };
     auto qk = [&](int t) {
-        const char* tile = lds + (t & 1) * kBuf;
-        auto frag = [&](int i) { return *reinterpret_cast<const f16x8*>(tile + k_addr<D>(2 * (i >> 1) + hh, 32 * (i & 1) + col)); };
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+        const char* tile = lds + (t & 1) * kBuf + k_addr<D>(hh, col);
+        auto frag = [&](int i) {  // chunk 2 (i / 2) + hh, keys 32 (i % 2) + col
+            return *reinterpret_cast<const f16x8*>(tile + (i >> 1) * (2 * kTile * 16) + (i & 1) * 512);
+        };
+        s[0] = f32x16{};
+        s[1] = f32x16{};
         f16x8 f[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) f[i] = frag(i);
 #pragma unroll
         for (int i = 0; i < 2 * KS; ++i) {
-#pragma unroll
-            for (int h = 0; h < PREC; ++h)
-                s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % kAhead], q[h][i >> 1], s[i & 1], 0, 0, 0);
+            const f16x8 kf = f[i % kAhead];
             if (i + kAhead < 2 * KS) f[i % kAhead] = frag(i + kAhead);
-            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int h = 0; h < PREC; ++h) s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[h][i >> 1], s[i & 1], 0, 0, 0);
         }
+        paced(2 * KS);
     };
     auto pv = [&](int t) {
-        const char* tile = lds + (2 + (t & 1)) * kBuf;
-        auto frag = [&](int i) { return *reinterpret_cast<const f16x8*>(tile + v_addr<D>(i / NB, hh, 32 * (i % NB) + col)); };
+        // page i / NB, half hh, channel (32 (i % NB) + col) ^ 16 hh
+        const char* tile = lds + (2 + (t & 1)) * kBuf + v_addr<D>(0, hh, col);
+        auto frag = [&](int i) { return *reinterpret_cast<const f16x8*>(tile + (i / NB) * (2 * D * 16) + (i % NB) * 512); };
         f16x8 f[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) f[i] = frag(i);
 #pragma unroll
         for (int i = 0; i < 4 * NB; ++i) {
+            const f16x8 vf = f[i % kAhead];
+            if (i + kAhead < 4 * NB) f[i % kAhead] = frag(i + kAhead);
 #pragma unroll
             for (int h = 0; h < PREC; ++h)
-                o[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[i % kAhead], pf[h][i / NB], o[i % NB], 0, 0, 0);
-            if (i + kAhead < 4 * NB) f[i % kAhead] = frag(i + kAhead);
-            __builtin_amdgcn_sched_barrier(0);
+                o[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[h][i / NB], o[i % NB], 0, 0, 0);
         }
+        paced(4 * NB);
     };
     // P of the tile against m, its sum over the lane's 32 keys.
     auto exps = [&] {
-        float sum = 0.f;
+        float part[4];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int st = 0; st < 4; ++st) {
+            float p[8];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int i = 0; i < 8; ++i) p[i] = fast_exp2(fmaf(s[st >> 1][8 * (st & 1) + i], back, -m));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float p = fast_exp2(fmaf(s[kb][8 * u + i], back, -m));
-                    sum += p;
-                    const int at = (i & 4) | ((i & 1) << 1) | ((i >> 1) & 1);  // 0, 2, 1, 3 of each four
-                    const f16 h = to_f16(p);
-                    pf[0][2 * kb + u][at] = h;
-                    if (PREC == 2) pf[PREC - 1][2 * kb + u][at] = to_f16(p - (float)h);
-                }
-        return sum;
+            for (int i = 0; i < 8; ++i) {
+                const float x = p[(i & 4) | ((i & 1) << 1) | ((i >> 1) & 1)];  // 0, 2, 1, 3 of each four: the V words' order
+                const f16 h = to_f16(x);
+                pf[0][st][i] = h;
+                if (PREC == 2) pf[PREC - 1][st][i] = to_f16(x - (float)h);
+            }
+            part[st] = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        }
+        return (part[0] + part[1]) + (part[2] + part[3]);
     };
     auto softmax = [&](int t, uint32_t bad) {
         if (bad != 0 || (t + 1) * kTile > lim_all) {  // scores that do not count: -inf after the factor, which is not 0
@@ -253,7 +269,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
                     if (32 * kb + 8 * (e >> 2) + (e & 3) >= left || ((bad >> (2 * kb + (e >> 3))) & 1)) s[kb][e] = none;
         }
         float sum = exps();
-        while (__any(sum > kRedo)) {  // at most once: no P is above 1 after it
+        if (__any(sum > kRedo)) {  // no P is above 1 after it
             float mx = -1e30f;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
@@ -292,18 +308,24 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         typedef T t4 __attribute__((ext_vector_type(4)));
         T* out = static_cast<T*>(a.out) + row * D + 4 * hh;
-        const T* gate = a.gate ? static_cast<const T*>(a.gate) + row * D + 4 * hh : nullptr;
+        if (a.gate) {
+            const T* gate = static_cast<const T*>(a.gate) + row * D + 4 * hh;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const t4 g = *reinterpret_cast<const t4*>(gate + 32 * nb + 8 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nb][4 * i + e] *= sigmoidf_(to_f32(g[e]));
+                }
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 t4 y;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = o[nb][4 * i + e] * inv;
-                    if (gate) v *= sigmoidf_(to_f32(gate[32 * nb + 8 * i + e]));
-                    y[e] = from_f32<T>(v);
-                }
+                for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(o[nb][4 * i + e] * inv);
                 *reinterpret_cast<t4*>(out + 32 * nb + 8 * i) = y;
             }
     };
