@@ -2034,8 +2034,9 @@ int pi_q4_pool_create(pi_handle h, int32_t n_pages, int32_t page_tokens, int32_t
     p->owner = h;
     p->bytes = (size_t)n_pages * n_kv_heads * pi::q4_block_bytes(head_dim);
     void* base = nullptr;
-    hipError_t e = hipMalloc(&base, p->bytes);
-    if (e == hipSuccess) e = hipMemset(base, 0, p->bytes);  // scales of 0: unwritten slots hold zeros
+    // 128 spare bytes: the attention's loads of a D 64 block end past it
+    hipError_t e = hipMalloc(&base, p->bytes + 128);
+    if (e == hipSuccess) e = hipMemset(base, 0, p->bytes + 128);  // scales of 0: unwritten slots hold zeros
     if (e != hipSuccess) {
         (void)hipFree(base);
         delete p;

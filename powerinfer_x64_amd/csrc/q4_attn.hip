@@ -32,10 +32,41 @@ constexpr int kWaves = sched::kWaves;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLazy = 8.0f;     // log2 headroom before the running max moves
 constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
-constexpr int kStage = 2048;      // floats a wavefront stages at a time for the merge in LDS
+constexpr int kStage = 2048;      // most floats a wavefront stages at a time for the merge in LDS
 constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
 constexpr long long kWholeBytes = 96 << 10;
 constexpr int kItemPages = 16;    // most pages of a work item
+
+// Pages on their way: each wavefront keeps a ring of whole (page, KV head) blocks in LDS, filled by direct loads
+// (no registers, no LDS stores) several pages ahead of the pair it works on.
+template <int D>
+struct Ring {
+    static constexpr int kBytes = 18 * D;                       // a block, copied as it lies
+    static constexpr int kWide = kBytes / 1024, kNarrow = (kBytes % 1024 + 255) / 256;  // 16- and 4-byte loads of 64 lanes
+    static constexpr int kSlot = kWide * 1024 + kNarrow * 256;  // D 64: the last load reads half a load past the block
+    static constexpr int kLoads = kWide + kNarrow;
+    static constexpr int kPages = D == 256 ? 4 : 8;             // slots: a pair at work, the others in flight
+};
+
+static_assert(kStage * 4 <= Ring<64>::kPages * Ring<64>::kSlot && kStage * 4 <= Ring<256>::kPages * Ring<256>::kSlot, "O is staged in the rings");
+
+// Global to LDS: lane l's 16 (4) bytes from base + off to dst + 16 l (4 l).  From assembly so that the compiler adds no waits
+// before LDS reads of other slots; M0 (the destination) is saved, the base and the destination are wave-uniform.
+__device__ __forceinline__ void dma16(const char* base, uint32_t off, uint32_t dst) {
+    uint32_t saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved)
+                 : "v"(off), "s"(base), "s"(dst)
+                 : "memory");
+}
+__device__ __forceinline__ void dma4(const char* base, uint32_t off, uint32_t dst) {
+    uint32_t saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(saved)
+                 : "v"(off), "s"(base), "s"(dst)
+                 : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 // A page of one KV head as a lane holds it.
 template <int D>
@@ -253,14 +284,20 @@ struct LenOf {
     __device__ __forceinline__ int operator()(int b) const { return rows_of(a, b).len; }
 };
 
+// Two wavefronts a SIMD where the rows' registers allow it.
 template <typename T, int D, int NCB>
-__global__ __launch_bounds__(kThreads) void q4_attn_kernel(Q4AttnArgs a, Q4Ws ws, int stage) {
-    extern __shared__ __attribute__((aligned(16))) float s_dyn[];  // [4][stage] staged O, then s_cum[batch + 1]
+constexpr int min_waves() { return NCB * D * (sizeof(T) == 4 ? 3 : 2) <= 512 ? 2 : 1; }
+
+template <typename T, int D, int NCB>
+__global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_kernel(Q4AttnArgs a, Q4Ws ws, int stage) {
+    typedef Ring<D> R;
+    // the wavefronts' rings, then s_cum[batch + 1]; the rings' space also stages O: [4][stage] floats
+    extern __shared__ __attribute__((aligned(16))) char s_dyn[];
     __shared__ int s_red[4];
     __shared__ float s_m[kWaves][16 * NCB];
     __shared__ float s_l[kWaves][16 * NCB];
-    float* s_o = s_dyn;
-    int* s_cum = reinterpret_cast<int*>(s_dyn + kWaves * stage);
+    float* s_o = reinterpret_cast<float*>(s_dyn);
+    int* s_cum = reinterpret_cast<int*>(s_dyn + kWaves * R::kPages * R::kSlot);
 
     const Q4Magic mg;
     const int n_kv = a.g.n_kv_heads, n_seg = n_kv * a.n_cb, tid = threadIdx.x;
@@ -280,6 +317,8 @@ __global__ __launch_bounds__(kThreads) void q4_attn_kernel(Q4AttnArgs a, Q4Ws ws
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
     const size_t blk_bytes = q4_block_bytes(D);
+    const char* ring = s_dyn + wave * (R::kPages * R::kSlot);
+    const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)ring);
 
     int b = sched::find_seq(s_cum, a.batch, n_seg, cur);
     while (cur < end) {
@@ -323,40 +362,50 @@ __global__ __launch_bounds__(kThreads) void q4_attn_kernel(Q4AttnArgs a, Q4Ws ws
             const bool bad = !sched::page_ok(pid_raw, a.g.n_pages);
             const int pid_v = bad ? 0 : pid_raw;
             const uint64_t bad_pages = __ballot(bad);
-            const int first_pid = __builtin_amdgcn_readfirstlane(pid_v);
-            auto load_pair = [&](Page<D>* dst, int i) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int j = 2 * i + u;
-                    const int pid = j < n_my ? __builtin_amdgcn_readlane(pid_v, j) : first_pid;
-                    dst[u].load(a.g.base + ((size_t)pid * n_kv + kvh) * blk_bytes, lane);
-                }
-            };
             constexpr int kNone = 0x7fffffc0;  // a page whose tokens are past every limit
-            auto run_pair = [&](const Page<D>* pg, int i) {
+            // page j of the wavefront's into its slot (its last reads are done: lgkmcnt 0)
+            auto issue = [&](int j) {
+                const int pid = __builtin_amdgcn_readlane(pid_v, j);
+                const char* blk = a.g.base + ((size_t)pid * n_kv + kvh) * blk_bytes;
+                const uint32_t dst = ring_at + (j % R::kPages) * R::kSlot;
+#pragma unroll
+                for (int i = 0; i < R::kWide; ++i) dma16(blk, i * 1024 + lane * 16, dst + i * 1024);
+#pragma unroll
+                for (int i = 0; i < R::kNarrow; ++i) dma4(blk, R::kWide * 1024 + i * 256 + lane * 4, dst + R::kWide * 1024 + i * 256);
+            };
+            const int n_iter = (n_my + 1) / 2;
+            for (int j = 0; j < min(n_my, R::kPages); ++j) issue(j);
+            for (int i = 0; i < n_iter; ++i) {
+                // this pair has landed; the younger ones may still be under way
+                constexpr int kAhead = R::kPages - 2;
+                const int ahead = n_my - 2 * i - 2;  // pages behind the pair
+                if (ahead >= kAhead)
+                    wait_loads<kAhead * R::kLoads>();
+                else if (kAhead > 4 && ahead >= 4)
+                    wait_loads<4 * R::kLoads>();
+                else if (kAhead > 2 && ahead >= 2)
+                    wait_loads<2 * R::kLoads>();
+                else
+                    wait_loads<0>();
+                Page<D> pg[2];
                 int tok0[2];
                 bool edge = false;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int j = 2 * i + u;
+                    const bool in = j < n_my;  // a pair's second page may not exist: the first, masked, in its place
+                    pg[u].load(ring + ((in ? j : 2 * i) % R::kPages) * R::kSlot, lane);
                     const int t = (first + kWaves * j) * sched::kPage;
-                    const bool on = j < n_my && !((bad_pages >> j) & 1);
+                    const bool on = in && !((bad_pages >> j) & 1);
                     tok0[u] = on ? t : kNone;
                     edge = edge || !on || t + sched::kPage > first_lim;
                 }
                 process<T, D, NCB>(acc, pg, q, back, lim, tok0, edge, grp, mg);
-            };
-            const int n_iter = (n_my + 1) / 2;
-            if (n_iter > 0) {
-                Page<D> now[2], next[2];
-                load_pair(now, 0);
-                for (int i = 0; i < n_iter - 1; ++i) {
-                    load_pair(next, i + 1);
-                    run_pair(now, i);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) now[u] = next[u];
+                if (2 * i + R::kPages < n_my) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    issue(2 * i + R::kPages);
+                    if (2 * i + 1 + R::kPages < n_my) issue(2 * i + 1 + R::kPages);
                 }
-                run_pair(now, n_iter - 1);
             }
         }
         // ---- the 4 wavefronts' shares meet in LDS, `stage` floats of rows at a time ----
@@ -370,6 +419,7 @@ __global__ __launch_bounds__(kThreads) void q4_attn_kernel(Q4AttnArgs a, Q4Ws ws
             }
         }
         const size_t slot = (size_t)sched::run_slot(cur == run.seg0, b, sidx, n_seg, a.batch, blockIdx.x);
+        __syncthreads();  // the rings are read no more
         const int per = stage / D;  // rows staged at a time: a power of two up to 16
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
@@ -520,6 +570,10 @@ int wgs_of(int d, int ncb) {
     return ncb == 1 ? vgpr_wgs<T, 64, 1>() : ncb == 2 ? vgpr_wgs<T, 64, 2>() : vgpr_wgs<T, 64, 4>();
 }
 
+size_t ring_bytes(int d) {
+    return kWaves * (d == 64 ? (size_t)Ring<64>::kPages * Ring<64>::kSlot
+                             : d == 128 ? (size_t)Ring<128>::kPages * Ring<128>::kSlot : (size_t)Ring<256>::kPages * Ring<256>::kSlot);
+}
 int stage_floats(int cols, int d) {  // rows staged at a time: a power of two, at most 16
     int per = std::min(16, kStage / d);
     while (per > 1 && per / 2 >= cols) per /= 2;
@@ -535,7 +589,13 @@ hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStrea
         ws.runs = reinterpret_cast<int32_t*>(ws.ml + (size_t)plan.n_slots * a.cols * 2);
     }
     const int stage = stage_floats(a.cols, D);
-    const size_t lds = (size_t)kWaves * stage * 4 + (size_t)(a.batch + 1) * 4;
+    const size_t lds = ring_bytes(D) + (size_t)(a.batch + 1) * 4;
+    if (lds > (64 << 10)) {  // more than a kernel may ask for without saying so
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_attn_kernel<T, D, NCB>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                        (int)(ring_bytes(D) + (kQ4MaxBatch + 1) * 4));
+        if (e != hipSuccess) return e;
+    }
     hipLaunchKernelGGL((q4_attn_kernel<T, D, NCB>), dim3(plan.grid), dim3(kThreads), lds, s, a, ws, stage);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -591,7 +651,7 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     a.cols = (int)std::min<long long>(rows, 16 * p.ncb);
     const int n_seg = n_kv * a.n_cb;
     const int regs = a.dtype == 0 ? wgs_of<float>(d, p.ncb) : a.dtype == 1 ? wgs_of<f16>(d, p.ncb) : wgs_of<bf16>(d, p.ncb);
-    const size_t lds = (size_t)kWaves * stage_floats(a.cols, d) * 4 + (size_t)(a.batch + 1) * 4 + 1024;
+    const size_t lds = ring_bytes(d) + (size_t)(a.batch + 1) * 4 + 2048;
     const int per_cu = std::max(1, std::min<int>(regs, (int)((160 << 10) / lds)));
     p.grid = std::min(cus * per_cu, kMaxRuns - 1);
     // Items of 16 pages, halved while the launch's most items would not give every workgroup two.
