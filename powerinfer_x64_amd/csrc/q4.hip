@@ -22,7 +22,9 @@ namespace pi {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTable = 256;  // (token, pair) angles of a workgroup
+constexpr int kTable = 512;     // (token, pair) angles of a workgroup
+constexpr int kMaxToks = 8;     // tokens of a workgroup
+constexpr int kManyRows = 1024; // rows from which a workgroup takes several tokens
 
 __device__ __forceinline__ double shfl_xor(double v, int m) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -64,15 +66,14 @@ __device__ __forceinline__ float group_scale(double m) {
 }
 
 // Quantises 8 consecutive channels of a row: every lane of the group's 4 holds 8.  Packed codes (nibble e:
-// channel e) and the group's scale.  NaN counts as 0; values past 8192 (and infinities) as 8192,
-// over the largest that the format holds.
+// channel e) and the group's scale.  NaN counts as 0; infinities, and what lies past the largest value that the format
+// holds, saturate.
 template <typename R>
-__device__ __forceinline__ uint32_t quantise8(const R* xin, float* scale) {
+__device__ __forceinline__ uint32_t quantise8(const R* x, float* scale) {
     typedef Real<R> F;
-    R x[8], hi = 0, lo = 0;
+    R hi = 0, lo = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        x[e] = xin[e] > (R)8192 ? (R)8192 : xin[e] < (R)-8192 ? (R)-8192 : xin[e];
         hi = F::max_(hi, x[e]);
         lo = F::min_(lo, x[e]);
     }
@@ -88,9 +89,8 @@ __device__ __forceinline__ uint32_t quantise8(const R* xin, float* scale) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         // x / s to the last bit that matters: a quotient that is a tie (k + 1/2) is exact after the correction
-        R t = x[e] * inv;
-        t = F::fma_(F::fma_(-t, sr, x[e]), inv, t);
-        t = F::rint_(t);
+        R t = F::min_(F::max_(x[e] * inv, (R)-9), (R)8);
+        t = F::rint_(F::fma_(F::fma_(-t, sr, x[e]), inv, t));
         const int c = t == t ? (int)F::min_(F::max_(t, (R)-8), (R)7) : 0;
         w |= (uint32_t)(c + 8) << (4 * e);
     }
@@ -121,211 +121,327 @@ struct Place {
     int slot;
 };
 
-// Norm and rotation of channels d0 .. d0 + 7 of a row (LPR lanes hold the row).
-template <typename T, typename R, bool VEC>
-__device__ __forceinline__ void norm_rotate(const T* row, int d0, int D, int lpr, const float* w, float eps, int half, int layout,
-                                            const double2* cs, R* y) {
-    typedef Real<R> F;
-    T xt[8], pt[8];
-    load_row8<T, VEC>(row + d0, xt);
-    const bool turn = layout == 1 && d0 < 2 * half;
-    // halves: the partners sit half a rotation away
-    if (turn) {
+// A lane's 16 channels of a row: two chunks of 8, at a and b.  With the halves layout a rotating chunk's partners are the
+// other chunk; in either layout four neighbouring lanes hold a group of 32 channels in each chunk.  (VEC: the widths divide
+// so, rows of 16-byte chunks.  Otherwise a lane has one chunk, and reads its partners for itself.)
+struct Chunks {
+    int a, b;
+    bool turn;  // halves: the two chunks rotate together
+};
+template <bool VEC>
+__device__ __forceinline__ Chunks chunks_of(int c, int D, int half, int layout) {
+    if (!VEC) return {8 * c, 8 * c, false};
+    if (layout != 1 || half == 0) return {8 * c, 8 * c + D / 2, false};
+    if (8 * c < half) return {8 * c, 8 * c + half, true};
+    const int o = half + 8 * c;  // 2 half + 8 (c - half / 8)
+    return {o, o + (D - 2 * half) / 2, false};
+}
+
+template <typename T, bool VEC>
+struct Raw {
+    T x[8], y[8];  // the chunks at a and b (VEC); the chunk and its partners
+    __device__ __forceinline__ void load(const T* row, const Chunks& ch, int half, int layout) {
+        load_row8<T, VEC>(row + ch.a, x);
         if (VEC)
-            load_row8<T, true>(row + (d0 < half ? d0 + half : d0 - half), pt);
-        else
+            load_row8<T, true>(row + ch.b, y);
+        else if (layout == 1 && ch.a < 2 * half)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int d = d0 + e;
-                pt[e] = row[d < half ? d + half : d < 2 * half ? d - half : d];
+                const int d = ch.a + e;
+                y[e] = row[d < half ? d + half : d < 2 * half ? d - half : d];
             }
     }
-    R x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = (R)to_f32(xt[e]);
-    R rs = 1;
-    if (w) {
-        R ss = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-        for (int m = 1; m < lpr; m <<= 1) ss += shfl_xor(ss, m);
-        rs = F::inv_sqrt(ss / (R)D + (R)eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * rs * (R)w[d0 + e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = x[e];
-    if (layout == 0) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            if (d0 + e >= 2 * half) break;
-            const double2 a = cs[(d0 + e) >> 1];
-            y[e] = x[e] * (R)a.x - x[e + 1] * (R)a.y;
-            y[e + 1] = x[e] * (R)a.y + x[e + 1] * (R)a.x;
-        }
-    } else if (turn) {
+};
+
+// The norm's weights of a lane's channels, the same for all of its rows: in registers, so that the loop over the rows waits for
+// nothing but the rows.
+struct Weights {
+    float x[8], y[8];
+    bool on;
+    template <bool VEC>
+    __device__ __forceinline__ void load(const float* w, const Chunks& ch, int half, int layout) {
+        on = w != nullptr;
+        if (!on) return;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const int d = d0 + e;
+            const int d = ch.a + e;
+            x[e] = w[d];
+            y[e] = VEC ? w[ch.b + e] : layout == 1 && d < 2 * half ? w[d < half ? d + half : d - half] : 0.f;
+        }
+    }
+};
+
+// Norm and rotation of a lane's channels; lpr lanes hold the row.  cs: cos and sin of the token's pairs.  u, v: the chunks
+// (v: VEC only).
+template <typename T, typename R, typename R2, bool VEC>
+__device__ __forceinline__ void norm_rotate(const Raw<T, VEC>& raw, const Chunks& ch, int D, int lpr, const Weights& w, float eps, int half,
+                                            int layout, const R2* cs, R* u, R* v) {
+    typedef Real<R> F;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        u[e] = (R)to_f32(raw.x[e]);
+        v[e] = (R)to_f32(raw.y[e]);
+    }
+    if (w.on) {
+        R ss = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += VEC ? u[e] * u[e] + v[e] * v[e] : u[e] * u[e];
+        for (int m = 1; m < lpr; m <<= 1) ss += shfl_xor(ss, m);
+        const R rs = F::inv_sqrt(ss / (R)D + (R)eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            u[e] = u[e] * rs * (R)w.x[e];
+            v[e] = v[e] * rs * (R)w.y[e];
+        }
+    }
+    if (layout == 0) {
+        auto pairs = [&](R* z, int d0) {
+            if (d0 >= 2 * half) return;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                if (!VEC && d0 + e >= 2 * half) break;
+                const R2 a = cs[(d0 + e) >> 1];
+                const R x0 = z[e], x1 = z[e + 1];
+                z[e] = x0 * a.x - x1 * a.y;
+                z[e + 1] = x0 * a.y + x1 * a.x;
+            }
+        };
+        pairs(u, ch.a);
+        if (VEC) pairs(v, ch.b);
+    } else if (VEC) {
+        if (!ch.turn) return;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const R2 a = cs[ch.a + e];
+            const R x0 = u[e], x1 = v[e];
+            u[e] = x0 * a.x - x1 * a.y;
+            v[e] = x0 * a.y + x1 * a.x;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int d = ch.a + e;
             if (d >= 2 * half) break;
             const bool first = d < half;
-            const int pd = first ? d + half : d - half;
-            R p = (R)to_f32(pt[e]);
-            if (w) p = p * rs * (R)w[pd];
-            const double2 a = cs[first ? d : pd];
-            y[e] = first ? x[e] * (R)a.x - p * (R)a.y : p * (R)a.y + x[e] * (R)a.x;
+            const R2 a = cs[first ? d : d - half];
+            u[e] = first ? u[e] * a.x - v[e] * a.y : v[e] * a.y + u[e] * a.x;
         }
     }
 }
 
-// The sequence and page of each of a workgroup's tokens, found by one wavefront: a sample of 64 of the
-// sequences' starts, then the 64 between two samples.  The tables are read, not trusted: a row is placed only
-// where its sequence's range holds it, as the attentions read it.
-__device__ __forceinline__ void find_places(const Q4AppendArgs& a, int row0, int n, Place* out) {
-    const int lane = threadIdx.x;
-    const int per = (a.n_seq + 63) / 64;
-    const int top = a.tok_start ? a.tok_start[min((lane + 1) * per, a.n_seq)] : 0;
-    for (int i = 0; i < n; ++i) {
-        const int row = row0 + i;
-        int s = row, first = row;
-        bool in = row < a.n_rows;
-        if (a.tok_start) {
-            const int blk = min((int)__popcll(__ballot((lane + 1) * per <= a.n_seq && top <= row)) * per, a.n_seq);
-            const int j = blk + 1 + lane;
-            s = blk;
-            if (per > 1) s += __popcll(__ballot(lane < per && j <= a.n_seq && a.tok_start[min(j, a.n_seq)] <= row));
-            in = in && s < a.n_seq;
-            s = min(s, a.n_seq - 1);
-            first = max(a.tok_start[s], 0);
-            in = in && row >= first && row < a.tok_start[s + 1];
-        }
-        const long long pos = (long long)max(a.start_pos[s], 0) + (row - first);
-        const long long lp = pos / sched::kPage;
-        int page = -1;
-        if (in && lp < a.max_pages) page = a.page_table[(size_t)s * a.max_pages + lp];
-        if (lane == 0) {
-            out[i].pos = in ? pos : -1;
-            out[i].page = page < a.g.n_pages ? page : -1;
-            out[i].slot = (int)(pos % sched::kPage);
+// The sequence and page of each of a workgroup's tokens, found by one wavefront: the token's place among a sample of 64 of
+// the sequences' starts, then among the 64 between two samples; the rest a lane a token.  The tables are read, not
+// trusted: a row is placed only where its sequence's range holds it, as the attentions read it.
+__device__ __forceinline__ void find_places(const Q4AppendArgs& a, int row0, int n, Place* out, bool pages) {
+    const int lane = threadIdx.x, row = row0 + lane;
+    int s = row;
+    if (a.tok_start) {
+        const int per = (a.n_seq + 63) / 64;
+        const int top = a.tok_start[min((lane + 1) * per, a.n_seq)];
+        for (int i = 0; i < n; ++i) {
+            int k = min((int)__popcll(__ballot((lane + 1) * per <= a.n_seq && top <= row0 + i)) * per, a.n_seq);
+            if (per > 1) {
+                const int j = k + 1 + lane;
+                k += __popcll(__ballot(lane < per && j <= a.n_seq && a.tok_start[min(j, a.n_seq)] <= row0 + i));
+            }
+            if (lane == i) s = k;
         }
     }
+    if (lane >= n) return;
+    bool in = s < a.n_seq;
+    s = min(s, a.n_seq - 1);
+    const int start = a.start_pos[s];
+    int first = row;
+    if (a.tok_start) {
+        first = max(a.tok_start[s], 0);
+        in = in && row >= first && row < a.tok_start[s + 1];
+    }
+    const long long pos = (long long)max(start, 0) + (row - first);
+    const long long lp = pos / sched::kPage;
+    int page = -1;
+    if (pages && in && lp < a.max_pages) page = a.page_table[(size_t)s * a.max_pages + lp];
+    out[lane].pos = in ? pos : -1;
+    out[lane].page = page < a.g.n_pages ? page : -1;
+    out[lane].slot = (int)(pos % sched::kPage);
 }
 
-// A workgroup: `toks` tokens (their angles fit the table), blockIdx.y: a share of their head rows.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(kThreads) void q4_append_kernel(Q4AppendArgs a, int toks) {
+__device__ __forceinline__ void store8(T* out, const float* y) {
+    if (VEC) {
+        constexpr int W = 16 / sizeof(T);
+        typedef T tv __attribute__((ext_vector_type(W)));
+#pragma unroll
+        for (int j = 0; j < 8 / W; ++j) {
+            tv r;
+#pragma unroll
+            for (int i = 0; i < W; ++i) r[i] = from_f32<T>(y[W * j + i]);
+            *reinterpret_cast<tv*>(out + W * j) = r;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = from_f32<T>(y[e]);
+    }
+}
+
+// A lane's channels of a query row: normed, rotated, written in the rows' type.
+template <typename T, bool VEC>
+__device__ __forceinline__ void put_q(const Q4AppendArgs& a, const Raw<T, VEC>& raw, const Weights& w, int row, int h, const Chunks& ch,
+                                      int lpr, const float2* cs) {
+    float u[8], v[8];
+    norm_rotate<T, float, float2, VEC>(raw, ch, a.g.head_dim, lpr, w, a.eps, a.plan.half, a.plan.layout, cs, u, v);
+    T* out = static_cast<T*>(a.q_out.p) + row * a.q_out.tok + h * a.q_out.head;
+    store8<T, VEC>(out + ch.a, u);
+    if (VEC) store8<T, VEC>(out + ch.b, v);
+}
+
+// A chunk's codes w and scale s to its page, and its values to where the caller wants them.
+__device__ __forceinline__ void put_codes(const Q4AppendArgs& a, uint32_t w, float s, bool is_v, int row, int kh, int d0, const Place& pl) {
+    const int D = a.g.head_dim, hkv = a.g.n_kv_heads, c = d0 >> 3;
+    uint16_t* val = is_v ? a.v_val : a.k_val;
+    if (val) {
+        typedef f16 h8 __attribute__((ext_vector_type(8)));
+        h8 r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = (f16)(s * (float)((int)((w >> (4 * e)) & 15u) - 8));
+        *reinterpret_cast<h8*>(val + ((size_t)row * hkv + kh) * D + d0) = r;
+    }
+    const uint32_t other = __shfl_xor(w, 2, 64);  // the channels 16 further on, or 16 before
+    if (pl.page < 0) return;
+    char* blk = a.g.base + ((size_t)pl.page * hkv + kh) * q4_block_bytes(D);
+    const uint16_t sb = __builtin_bit_cast(uint16_t, (f16)s);
+    const int j = c >> 2, i4 = c & 3;
+    if (!is_v) {
+        uint32_t k = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k |= ((w >> (4 * e)) & 15u) << (4 * ((e >> 1) + 4 * (e & 1)));
+        *reinterpret_cast<uint32_t*>(blk + q4_k_off(D, pl.slot, c)) = k;
+        if (i4 == 0) *reinterpret_cast<uint16_t*>(blk + q4_ks_off(D, pl.slot, j)) = sb;
+    } else {
+        const uint32_t lo = i4 < 2 ? w : other, hi = i4 < 2 ? other : w;
+        const int m0 = 8 * (i4 & 1), e0 = i4 < 2 ? 0 : 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t b = ((lo >> (4 * (e0 + e))) & 15u) | (((hi >> (4 * (e0 + e))) & 15u) << 4);
+            *reinterpret_cast<uint8_t*>(blk + q4_v_off(D, pl.slot, j, m0 + e0 + e)) = (uint8_t)b;
+        }
+        if (i4 == 0) *reinterpret_cast<uint16_t*>(blk + q4_vs_off(D, pl.slot, j)) = sb;
+    }
+}
+
+// A lane's channels of a key or value row: normed and rotated (keys), quantised, stored.
+template <typename T, bool VEC>
+__device__ __forceinline__ void put_kv(const Q4AppendArgs& a, const Raw<T, VEC>& raw, const Weights& nw, bool is_v, int row, int kh,
+                                       const Chunks& ch, int lpr, const Place& pl, const double2* cs) {
+    float s0, s1 = 0.f;
+    uint32_t w0, w1 = 0;
+    if (!is_v) {
+        double u[8], v[8];
+        norm_rotate<T, double, double2, VEC>(raw, ch, a.g.head_dim, lpr, nw, a.eps, a.plan.half, a.plan.layout, cs, u, v);
+        w0 = quantise8<double>(u, &s0);
+        if (VEC) w1 = quantise8<double>(v, &s1);
+    } else {
+        typedef typename std::conditional<sizeof(T) == 4, double, float>::type R;
+        R u[8], v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            u[e] = (R)to_f32(raw.x[e]);
+            v[e] = (R)to_f32(raw.y[e]);
+        }
+        w0 = quantise8<R>(u, &s0);
+        if (VEC) w1 = quantise8<R>(v, &s1);
+    }
+    put_codes(a, w0, s0, is_v, row, kh, ch.a, pl);
+    if (VEC) put_codes(a, w1, s1, is_v, row, kh, ch.b, pl);
+}
+
+// Workgroups 0 .. kv_wgs - 1 take the keys and values of `toks` tokens each (f64 angles, quantiser), the others the
+// queries of `toks` tokens (f32): in one launch, so that the heavier arithmetic runs beside the larger share
+// of the bytes.  blockIdx.y: a share of the tokens' rows.  A workgroup's first rows are requested before it looks
+// up its tokens' places and computes their angles.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4) void q4_append_kernel(Q4AppendArgs a, int toks, int kv_wgs) {
     __shared__ double2 s_cs[kTable];
-    __shared__ Place s_place[4];
+    __shared__ Place s_place[kMaxToks];
     const int tid = threadIdx.x, D = a.g.head_dim, half = a.plan.half;
-    const int row0 = blockIdx.x * toks, n = min(toks, a.n_rows - row0);
-    if (tid < 64) find_places(a, row0, n, s_place);
+    const bool kv = (int)blockIdx.x < kv_wgs;
+    const int row0 = (kv ? blockIdx.x : blockIdx.x - kv_wgs) * toks, n = min(toks, a.n_rows - row0);
+    const int hkv = a.g.n_kv_heads, heads = kv ? 2 * hkv : a.q.n;
+    const int lpr = D / (VEC ? 16 : 8), rpi = kThreads / lpr;  // lanes a row, rows at a time
+    const int rl = tid / lpr;
+    const Chunks ch = chunks_of<VEC>(tid - rl * lpr, D, half, a.plan.layout);
+    const int step = gridDim.y * rpi;
+    int u = blockIdx.y * rpi + rl, t = u / heads, h = u - t * heads;
+    const T* const p0 = static_cast<const T*>(kv ? a.k.p : a.q.p);
+    const T* const p1 = static_cast<const T*>(a.v.p);
+    const int64_t tok0 = kv ? a.k.tok : a.q.tok, head0 = kv ? a.k.head : a.q.head, tok1 = a.v.tok, head1 = a.v.head;
+    auto load = [&](Raw<T, VEC>& r, int tt, int hh) {
+        if (tt >= n) return;
+        const bool is_v = kv && hh >= hkv;
+        const T* row = is_v ? p1 + (row0 + tt) * tok1 + (hh - hkv) * head1 : p0 + (row0 + tt) * tok0 + hh * head0;
+        r.load(row, ch, is_v ? 0 : half, a.plan.layout);
+    };
+    Raw<T, VEC> raw;
+    load(raw, t, h);
+    Weights w;
+    w.template load<VEC>(kv ? a.k_norm : a.q_norm, ch, half, a.plan.layout);
+    if (tid < 64) find_places(a, row0, n, s_place, kv);
     __syncthreads();
-    for (int i = tid; i < n * half; i += kThreads) {
-        const int t = i / half;
-        double turns = (double)s_place[t].pos * a.plan.turns[i - t * half];
-        turns -= rint(turns);
-        double sn, cn;
-        sincospi(2.0 * turns, &sn, &cn);
-        s_cs[i] = double2{cn * a.plan.mscale, sn * a.plan.mscale};
+    if (kv) {
+        for (int i = tid; i < n * half; i += kThreads) {
+            const int tt = i / half;
+            double turns = (double)s_place[tt].pos * a.plan.turns[i - tt * half];
+            turns -= rint(turns);
+            double sn, cn;
+            sincospi(2.0 * turns, &sn, &cn);
+            s_cs[i] = double2{cn * a.plan.mscale, sn * a.plan.mscale};
+        }
+    } else {
+        float2* f_cs = reinterpret_cast<float2*>(s_cs);
+        for (int i = tid; i < n * half; i += kThreads) {
+            const int tt = i / half;
+            double turns = (double)s_place[tt].pos * a.plan.turns[i - tt * half];
+            turns -= rint(turns);
+            float sn, cn;
+            sincospif((float)(2.0 * turns), &sn, &cn);
+            f_cs[i] = float2{cn * (float)a.plan.mscale, sn * (float)a.plan.mscale};
+        }
     }
     __syncthreads();
-    const int lpr = D / 8, rpi = kThreads / lpr;       // lanes a row, rows at a time
-    const int rl = tid / lpr, c = tid - rl * lpr, d0 = 8 * c;
-    const int hkv = a.g.n_kv_heads, heads = a.q.n + 2 * hkv;
-    for (int u = blockIdx.y * rpi + rl; u < n * heads; u += gridDim.y * rpi) {
-        const int t = u / heads, h = u - t * heads, row = row0 + t;
-        const Place pl = s_place[t];
-        if (pl.pos < 0) continue;  // uniform over a row's lanes
-        const double2* cs = s_cs + t * half;
-        if (h < a.q.n) {
-            const T* in = static_cast<const T*>(a.q.p) + row * a.q.tok + h * a.q.head;
-            T* out = static_cast<T*>(a.q_out.p) + row * a.q_out.tok + h * a.q_out.head;
-            float y[8];
-            norm_rotate<T, float, VEC>(in, d0, D, lpr, a.q_norm, a.eps, half, a.plan.layout, cs, y);
-            if (VEC) {
-                constexpr int W = 16 / sizeof(T);
-                typedef T tv __attribute__((ext_vector_type(W)));
-#pragma unroll
-                for (int j = 0; j < 8 / W; ++j) {
-                    tv r;
-#pragma unroll
-                    for (int i = 0; i < W; ++i) r[i] = from_f32<T>(y[W * j + i]);
-                    *reinterpret_cast<tv*>(out + d0 + W * j) = r;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) out[d0 + e] = from_f32<T>(y[e]);
-            }
-            continue;
-        }
-        const bool is_v = h >= a.q.n + hkv;
-        const int kh = h - a.q.n - (is_v ? hkv : 0);
-        float s;
-        uint32_t w;
-        if (!is_v) {
-            double y[8];
-            norm_rotate<T, double, VEC>(static_cast<const T*>(a.k.p) + row * a.k.tok + kh * a.k.head, d0, D, lpr, a.k_norm, a.eps,
-                                        half, a.plan.layout, cs, y);
-            w = quantise8<double>(y, &s);
-        } else {
-            typedef typename std::conditional<sizeof(T) == 4, double, float>::type R;
-            T xt[8];
-            R x[8];
-            load_row8<T, VEC>(static_cast<const T*>(a.v.p) + row * a.v.tok + kh * a.v.head + d0, xt);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (R)to_f32(xt[e]);
-            w = quantise8<R>(x, &s);
-        }
-        uint16_t* val = is_v ? a.v_val : a.k_val;
-        if (val) {
-            typedef f16 h8 __attribute__((ext_vector_type(8)));
-            h8 r;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) r[e] = (f16)(s * (float)((int)((w >> (4 * e)) & 15u) - 8));
-            *reinterpret_cast<h8*>(val + ((size_t)row * hkv + kh) * D + d0) = r;
-        }
-        const uint32_t other = __shfl_xor(w, 2, 64);  // the channels 16 further on, or 16 before
-        if (pl.page < 0) continue;
-        char* blk = a.g.base + ((size_t)pl.page * hkv + kh) * q4_block_bytes(D);
-        const uint16_t sb = __builtin_bit_cast(uint16_t, (f16)s);
-        const int j = c >> 2, i4 = c & 3;
-        if (!is_v) {
-            uint32_t k = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) k |= ((w >> (4 * e)) & 15u) << (4 * ((e >> 1) + 4 * (e & 1)));
-            *reinterpret_cast<uint32_t*>(blk + q4_k_off(D, pl.slot, c)) = k;
-            if (i4 == 0) *reinterpret_cast<uint16_t*>(blk + q4_ks_off(D, pl.slot, j)) = sb;
-        } else {
-            const uint32_t lo = i4 < 2 ? w : other, hi = i4 < 2 ? other : w;
-            const int m0 = 8 * (i4 & 1), e0 = i4 < 2 ? 0 : 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t b = ((lo >> (4 * (e0 + e))) & 15u) | (((hi >> (4 * (e0 + e))) & 15u) << 4);
-                *reinterpret_cast<uint8_t*>(blk + q4_v_off(D, pl.slot, j, m0 + e0 + e)) = (uint8_t)b;
-            }
-            if (i4 == 0) *reinterpret_cast<uint16_t*>(blk + q4_vs_off(D, pl.slot, j)) = sb;
-        }
+    while (t < n) {
+        const Raw<T, VEC> now = raw;
+        const int tn = t, hn = h;
+        u += step;
+        t = u / heads;
+        h = u - t * heads;
+        load(raw, t, h);
+        const Place pl = s_place[tn];
+        if (pl.pos < 0) continue;  // a row of no sequence; uniform over a row's lanes
+        if (kv)
+            put_kv<T, VEC>(a, now, w, hn >= hkv, row0 + tn, hn >= hkv ? hn - hkv : hn, ch, lpr, pl, s_cs + tn * half);
+        else
+            put_q<T, VEC>(a, now, w, row0 + tn, hn, ch, lpr, reinterpret_cast<const float2*>(s_cs) + tn * half);
     }
 }
 
 template <typename T>
 hipError_t launch_append_t(const Q4AppendArgs& a, hipStream_t s) {
     const int e = (int)sizeof(T), D = a.g.head_dim;
-    bool vec = a.plan.half % 8 == 0;
+    const int half = a.plan.half;
+    bool vec = a.plan.layout == 1 && half ? half % 32 == 0 && (D - 2 * half) % 64 == 0 : half % 4 == 0;
     for (const HeadRows* r : {&a.q, &a.q_out, &a.k, &a.v})
         if (r->p) vec = vec && reinterpret_cast<uintptr_t>(r->p) % 16 == 0 && r->tok * e % 16 == 0 && r->head * e % 16 == 0;
-    // Tokens of a workgroup: their angles fill the table in one pass; one token while the launch is small.
-    const int fit = a.plan.half ? std::max(1, kTable / a.plan.half) : 4;
-    const int toks = a.n_rows >= 1024 ? std::min(fit, 4) : 1;
-    const int rpi = kThreads * 8 / D, rows = toks * (a.q.n + 2 * a.g.n_kv_heads);
-    const long long wgs = (a.n_rows + toks - 1) / toks;
-    const int blocks = (rows + rpi - 1) / rpi;
-    const int y = wgs * blocks <= 2048 ? std::min(blocks, 65535) : 1;
-    const dim3 grid((unsigned)wgs, y);
+    // Tokens of a workgroup: as many as fill the angles' table in one pass of its threads; one while the launch is small.
+    const int fit = half ? std::max(1, kTable / half) : kMaxToks;
+    const int toks = a.n_rows >= kManyRows ? std::min(fit, kMaxToks) : 1;
+    const int rpi = kThreads * (vec ? 16 : 8) / D;
+    const long long wgs = (a.n_rows + toks - 1) / toks, all = wgs * (a.q.n ? 2 : 1);
+    const int blocks = (toks * std::max(a.q.n, 2 * a.g.n_kv_heads) + rpi - 1) / rpi;
+    const int y = all * blocks <= 2048 ? std::min(blocks, 65535) : 1;
+    const dim3 grid((unsigned)all, y);
     if (vec)
-        hipLaunchKernelGGL((q4_append_kernel<T, true>), grid, dim3(kThreads), 0, s, a, toks);
+        hipLaunchKernelGGL((q4_append_kernel<T, true>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
     else
-        hipLaunchKernelGGL((q4_append_kernel<T, false>), grid, dim3(kThreads), 0, s, a, toks);
+        hipLaunchKernelGGL((q4_append_kernel<T, false>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
     return hipGetLastError();
 }
 

@@ -35,6 +35,7 @@ constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
 constexpr int kStage = 2048;      // most floats a wavefront stages at a time for the merge in LDS
 constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
 constexpr long long kWholeBytes = 96 << 10;
+constexpr int kAlign = 8;         // grid workgroups a segment from which segments are cut into pieces of their own
 constexpr int kItemPages = 16;    // most pages of a work item
 
 // Pages on their way: each wavefront keeps a ring of whole (page, KV head) blocks in LDS, filled by direct loads
@@ -50,21 +51,36 @@ struct Ring {
 
 static_assert(kStage * 4 <= Ring<64>::kPages * Ring<64>::kSlot && kStage * 4 <= Ring<256>::kPages * Ring<256>::kSlot, "O is staged in the rings");
 
-// Global to LDS: lane l's 16 (4) bytes from base + off to dst + 16 l (4 l).  From assembly so that the compiler adds no waits
-// before LDS reads of other slots; M0 (the destination) is saved, the base and the destination are wave-uniform.
-__device__ __forceinline__ void dma16(const char* base, uint32_t off, uint32_t dst) {
+// A block into a slot: its bytes in order, 16 (the rest: 4) a lane and load.  An instruction's offset counts for
+// both addresses.  From assembly so that the compiler adds no waits before LDS reads of other slots; M0 (the
+// destination) is saved, blk and dst are wave-uniform, and the wavefront's reads of the slot are done first.
+template <int D>
+__device__ __forceinline__ void load_block(const char* blk, uint32_t dst, uint32_t lane16, uint32_t lane4) {
     uint32_t saved;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(saved)
-                 : "v"(off), "s"(base), "s"(dst)
-                 : "memory");
-}
-__device__ __forceinline__ void dma4(const char* base, uint32_t off, uint32_t dst) {
-    uint32_t saved;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(saved)
-                 : "v"(off), "s"(base), "s"(dst)
-                 : "memory");
+    if constexpr (D == 64)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
+                     "global_load_lds_dwordx4 %1, %3\n\t"
+                     "global_load_lds_dword %2, %3 offset:1024\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(saved) : "v"(lane16), "v"(lane4), "s"(blk), "s"(dst) : "memory");
+    else if constexpr (D == 128)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
+                     "global_load_lds_dwordx4 %1, %3\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:1024\n\t"
+                     "global_load_lds_dword %2, %3 offset:2048\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(saved) : "v"(lane16), "v"(lane4), "s"(blk), "s"(dst) : "memory");
+    else
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
+                     "global_load_lds_dwordx4 %1, %3\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:3072\n\t"
+                     "s_mov_b32 m0, %5\n\t"
+                     "global_load_lds_dword %2, %6\n\t"
+                     "global_load_lds_dword %2, %6 offset:256\n\t"
+                     "s_mov_b32 m0, %0"
+                     : "=&s"(saved) : "v"(lane16), "v"(lane4), "s"(blk), "s"(dst), "s"(dst + 4096), "s"(blk + 4096) : "memory");
 }
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
@@ -253,12 +269,13 @@ struct Q4Ws {
 };
 
 // Prefix sums of the sequences' items into s_cum; returns their total.
-__device__ __forceinline__ int scan_items(const Q4AttnArgs& a, int* s_cum, int* s_red) {
+// (of each count divided by `per`, rounded up, where per > 1).
+__device__ __forceinline__ int scan_items(const Q4AttnArgs& a, int* s_cum, int* s_red, int per) {
     const int tid = threadIdx.x;
     int carry = 0;
     for (int base = 0; base < a.batch; base += kThreads) {
         const int b = base + tid;
-        const int n = b < a.batch ? sched::items_of(rows_of(a, b).len, a.item_pages) : 0;
+        const int n = b < a.batch ? (sched::items_of(rows_of(a, b).len, a.item_pages) + per - 1) / per : 0;
         int x = n;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -308,8 +325,18 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
             T* out = static_cast<T*>(a.out) + (size_t)rw.first * a.n_q_heads * D;
             for (size_t i = tid; i < (size_t)rw.n * a.n_q_heads * D; i += kThreads) out[i] = from_f32<T>(0.f);
         }
-    const int n_items = n_seg * scan_items(a, s_cum, s_red);
-    const int chunk = (n_items + gridDim.x - 1) / gridDim.x;
+    int n_items = n_seg * scan_items(a, s_cum, s_red, 1);
+    int chunk = (n_items + gridDim.x - 1) / gridDim.x;
+    // Few segments for the grid: each is cut into pieces of its own instead, a piece a workgroup, so that none pays the
+    // start and the end of two runs.  Pieces of `piece` items number at most the grid.
+    const int segs = a.batch * n_seg;
+    int piece = 0;
+    if (ws.runs && segs * kAlign <= (int)gridDim.x) {
+        piece = max(1, (n_items + (int)gridDim.x - segs - 1) / ((int)gridDim.x - segs));
+        __syncthreads();
+        n_items = n_seg * scan_items(a, s_cum, s_red, piece);
+        chunk = 1;  // s_cum counts pieces now
+    }
     int cur = blockIdx.x * chunk;
     const int end = min(n_items, cur + chunk);
     if (cur >= end) return;
@@ -318,12 +345,19 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
     const int col = lane & 15, grp = lane >> 4;
     const size_t blk_bytes = q4_block_bytes(D);
     const char* ring = s_dyn + wave * (R::kPages * R::kSlot);
+    const uint32_t lane16 = lane * 16, lane4 = lane * 4;
     const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)ring);
 
     int b = sched::find_seq(s_cum, a.batch, n_seg, cur);
     while (cur < end) {
-        const sched::Run run = sched::run_of(s_cum, LenOf{a}, n_seg, a.item_pages, b, cur, end);
+        sched::Run run = sched::run_of(s_cum, LenOf{a}, n_seg, a.item_pages, b, cur, end);
         b = run.b;
+        if (piece) {  // the segment's pages in equal pieces
+            const int k = s_cum[b + 1] - s_cum[b], pages = (run.len + sched::kPage - 1) / sched::kPage;
+            const int i = cur - run.seg0, each = (pages + k - 1) / k;
+            run.pg0 = min(pages, i * each);
+            run.pg1 = min(pages, run.pg0 + each);
+        }
         const int sidx = run.kvh, kvh = sidx / a.n_cb, row0 = (sidx % a.n_cb) * a.cols;
         const Q4Rows rw = rows_of(a, b);
         const size_t seg = (size_t)b * n_seg + sidx;
@@ -338,22 +372,19 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
             continue;
         }
         const int first_lim = rw.start + row0 / a.group + 1;  // keys that every row of the block sees
+        const int32_t* pt = a.page_table + (size_t)b * a.max_pages;
         Query<T, D> q[NCB];
         Acc<D, NCB> acc;
         float back[NCB];
         int lim[NCB];
+        bool have_q = false;
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
-            const int r = cb * 16 + col;
-            const long long off = r < a.cols ? row_offset(a, rw, kvh, row0 + r, D) : -1;
-            back[cb] = q[cb].load(static_cast<const T*>(a.q), off, grp, a.scale);
-            lim[cb] = min(rw.start + (row0 + r) / a.group + 1, rw.len);
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) acc.o[cb][t] = f32x4{0.f, 0.f, 0.f, 0.f};
             acc.m[cb] = -1e30f;
             acc.l[cb] = 0.f;
         }
-        const int32_t* pt = a.page_table + (size_t)b * a.max_pages;
         for (int sub = run.pg0; sub < run.pg1; sub += sched::kSubPages) {
             int first, n_my;
             sched::sub_pages(sub, run.pg1, wave, &first, &n_my);
@@ -363,49 +394,63 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
             const int pid_v = bad ? 0 : pid_raw;
             const uint64_t bad_pages = __ballot(bad);
             constexpr int kNone = 0x7fffffc0;  // a page whose tokens are past every limit
-            // page j of the wavefront's into its slot (its last reads are done: lgkmcnt 0)
-            auto issue = [&](int j) {
+            auto issue = [&](int j) {  // page j of the wavefront's into its slot
                 const int pid = __builtin_amdgcn_readlane(pid_v, j);
-                const char* blk = a.g.base + ((size_t)pid * n_kv + kvh) * blk_bytes;
-                const uint32_t dst = ring_at + (j % R::kPages) * R::kSlot;
-#pragma unroll
-                for (int i = 0; i < R::kWide; ++i) dma16(blk, i * 1024 + lane * 16, dst + i * 1024);
-#pragma unroll
-                for (int i = 0; i < R::kNarrow; ++i) dma4(blk, R::kWide * 1024 + i * 256 + lane * 4, dst + R::kWide * 1024 + i * 256);
+                load_block<D>(a.g.base + ((size_t)pid * n_kv + kvh) * blk_bytes, ring_at + (j % R::kPages) * R::kSlot, lane16, lane4);
             };
-            const int n_iter = (n_my + 1) / 2;
             for (int j = 0; j < min(n_my, R::kPages); ++j) issue(j);
-            for (int i = 0; i < n_iter; ++i) {
-                // this pair has landed; the younger ones may still be under way
+            if (!have_q) {  // the rows, while the first pages are on their way
+                have_q = true;
+#pragma unroll
+                for (int cb = 0; cb < NCB; ++cb) {
+                    const int r = cb * 16 + col;
+                    const long long off = r < a.cols ? row_offset(a, rw, kvh, row0 + r, D) : -1;
+                    back[cb] = q[cb].load(static_cast<const T*>(a.q), off, grp, a.scale);
+                    lim[cb] = min(rw.start + (row0 + r) / a.group + 1, rw.len);
+                }
+            }
+            // pages 2 i and 2 i + 1 have landed; the younger ones may still be under way
+            auto landed = [&](int i) {
                 constexpr int kAhead = R::kPages - 2;
                 const int ahead = n_my - 2 * i - 2;  // pages behind the pair
-                if (ahead >= kAhead)
-                    wait_loads<kAhead * R::kLoads>();
-                else if (kAhead > 4 && ahead >= 4)
-                    wait_loads<4 * R::kLoads>();
-                else if (kAhead > 2 && ahead >= 2)
+                if (kAhead >= 6 && ahead >= 6)
+                    wait_loads<(kAhead >= 6 ? 6 : 0) * R::kLoads>();
+                else if (kAhead >= 4 && ahead >= 4)
+                    wait_loads<(kAhead >= 4 ? 4 : 0) * R::kLoads>();
+                else if (ahead >= 2)
                     wait_loads<2 * R::kLoads>();
                 else
                     wait_loads<0>();
-                Page<D> pg[2];
+            };
+            auto fetch = [&](Page<D>* pg, int i) {  // the pair to registers; a second page that does not exist: the first, masked
+#pragma unroll
+                for (int u = 0; u < 2; ++u) pg[u].load(ring + ((2 * i + u < n_my ? 2 * i + u : 2 * i) % R::kPages) * R::kSlot, lane);
+            };
+            auto run_pair = [&](const Page<D>* pg, int i) {
                 int tok0[2];
                 bool edge = false;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int j = 2 * i + u;
-                    const bool in = j < n_my;  // a pair's second page may not exist: the first, masked, in its place
-                    pg[u].load(ring + ((in ? j : 2 * i) % R::kPages) * R::kSlot, lane);
                     const int t = (first + kWaves * j) * sched::kPage;
-                    const bool on = in && !((bad_pages >> j) & 1);
+                    const bool on = j < n_my && !((bad_pages >> j) & 1);
                     tok0[u] = on ? t : kNone;
                     edge = edge || !on || t + sched::kPage > first_lim;
                 }
                 process<T, D, NCB>(acc, pg, q, back, lim, tok0, edge, grp, mg);
-                if (2 * i + R::kPages < n_my) {
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    issue(2 * i + R::kPages);
-                    if (2 * i + 1 + R::kPages < n_my) issue(2 * i + 1 + R::kPages);
-                }
+            };
+            auto refill = [&](int i) {  // the pair's slots, once it is in registers
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (2 * i + u + R::kPages < n_my) issue(2 * i + u + R::kPages);
+            };
+            const int n_iter = (n_my + 1) / 2;
+            for (int i = 0; i < n_iter; ++i) {
+                Page<D> x[2];
+                landed(i);
+                fetch(x, i);
+                run_pair(x, i);
+                refill(i);
             }
         }
         // ---- the 4 wavefronts' shares meet in LDS, `stage` floats of rows at a time ----
@@ -419,7 +464,23 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
             }
         }
         const size_t slot = (size_t)sched::run_slot(cur == run.seg0, b, sidx, n_seg, a.batch, blockIdx.x);
-        __syncthreads();  // the rings are read no more
+        __syncthreads();  // (the rings are read no more, either)
+        if (tid < a.cols) {  // each wavefront's weight, and the row's max and sum
+            float M = s_m[0][tid], lsum = 0.f;
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][tid]);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = fast_exp2(s_m[w][tid] - M);
+                lsum += f * s_l[w][tid];
+                s_m[w][tid] = f;
+            }
+            if (!run.whole) {
+                ws.ml[(slot * a.cols + tid) * 2] = M;
+                ws.ml[(slot * a.cols + tid) * 2 + 1] = lsum;
+            }
+            s_l[0][tid] = run.whole ? (lsum == 0.f ? 0.f : 1.0f / lsum) : 1.0f;  // every key masked: zeros (a NaN stays)
+        }
         const int per = stage / D;  // rows staged at a time: a power of two up to 16
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
@@ -432,32 +493,29 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
                         *reinterpret_cast<f32x4*>(&s_o[wave * stage + (col - c0) * D + 16 * t + 4 * grp]) = acc.o[cb][t];
                 }
                 __syncthreads();
-                for (int idx = tid; idx < per * D; idx += kThreads) {
+                for (int idx = 4 * tid; idx < per * D; idx += 4 * kThreads) {
                     const int c = idx / D, d = idx - c * D, r = r0 + c;
                     if (r >= a.cols) break;
-                    float M = s_m[0][r];
+                    f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][r]);
-                    float o = 0.f, lsum = 0.f;
+                    for (int w = 0; w < kWaves; ++w) o += s_m[w][r] * *reinterpret_cast<const f32x4*>(&s_o[w * stage + idx]);
+                    o *= s_l[0][r];
+                    if (!run.whole) {
+                        *reinterpret_cast<f32x4*>(&ws.o[(slot * a.cols + r) * D + d]) = o;
+                        continue;
+                    }
+                    const long long off = row_offset(a, rw, kvh, row0 + r, D);
+                    if (off < 0) continue;
+                    typedef T t4 __attribute__((ext_vector_type(4)));
+                    t4 y;
+                    if (a.gate) {
+                        const t4 g = *reinterpret_cast<const t4*>(static_cast<const T*>(a.gate) + off + d);
 #pragma unroll
-                    for (int w = 0; w < kWaves; ++w) {
-                        const float f = fast_exp2(s_m[w][r] - M);
-                        o += f * s_o[w * stage + idx];
-                        lsum += f * s_l[w][r];
+                        for (int e = 0; e < 4; ++e) o[e] *= sigmoidf_(to_f32(g[e]));
                     }
-                    if (run.whole) {
-                        const long long off = row_offset(a, rw, kvh, row0 + r, D);
-                        if (off < 0) continue;
-                        float y = lsum == 0.f ? 0.f : o / lsum;  // every key masked: zeros (a NaN stays)
-                        if (a.gate) y *= sigmoidf_(to_f32(static_cast<const T*>(a.gate)[off + d]));
-                        static_cast<T*>(a.out)[off + d] = from_f32<T>(y);
-                    } else {
-                        ws.o[(slot * a.cols + r) * D + d] = o;
-                        if (d == 0) {
-                            ws.ml[(slot * a.cols + r) * 2] = M;
-                            ws.ml[(slot * a.cols + r) * 2 + 1] = lsum;
-                        }
-                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(o[e]);
+                    *reinterpret_cast<t4*>(static_cast<T*>(a.out) + off + d) = y;
                 }
                 __syncthreads();
             }
@@ -654,10 +712,10 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     const size_t lds = ring_bytes(d) + (size_t)(a.batch + 1) * 4 + 2048;
     const int per_cu = std::max(1, std::min<int>(regs, (int)((160 << 10) / lds)));
     p.grid = std::min(cus * per_cu, kMaxRuns - 1);
-    // Items of 16 pages, halved while the launch's most items would not give every workgroup two.
+    // Items of 16 pages, halved while the launch's most items would not give every workgroup eight.
     const long long seg_pages = (long long)a.batch * n_seg * a.use_pages;
     int ip = kItemPages;
-    while (ip > 1 && seg_pages / ip < 2LL * p.grid) ip >>= 1;
+    while (ip > 1 && seg_pages / ip < 8LL * p.grid) ip >>= 1;
     // A short segment is one item: read by one workgroup in less time than a merge's launch takes.
     if ((long long)a.use_pages * q4_block_bytes(d) <= kWholeBytes) ip = std::max(ip, a.use_pages);
     a.item_pages = ip;
