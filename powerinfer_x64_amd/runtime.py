@@ -736,18 +736,37 @@ class RopePlan:
 
 def _rows(t: torch.Tensor, name: str, dtype, shape, dev):
     """A tensor of head rows [n, heads, D] at any strides of its first two dimensions: its address and them."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == dev:
+        st, sh, sd = t.stride()
+        if sd == 1 or shape[2] <= 1:
+            return t.data_ptr(), st, sh
+        raise InvalidArg(f"{name}: the last dimension must be contiguous")
     if not isinstance(t, torch.Tensor):
         raise InvalidArg(f"{name}: expected a torch.Tensor")
     if t.device != dev:
         raise InvalidArg(f"{name}: on {t.device}, expected {dev}")
     if t.dtype != dtype:
         raise InvalidArg(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if t.shape != shape:
-        raise InvalidArg(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    st, sh, sd = t.stride()
-    if sd != 1 and shape[2] > 1:
-        raise InvalidArg(f"{name}: the last dimension must be contiguous")
-    return t.data_ptr(), st, sh
+    raise InvalidArg(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+def _table(t: torch.Tensor, name: str, dtype, shape, dev):
+    """A contiguous tensor's address (None: None)."""
+    if t is None:
+        return None
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous()):
+        _need(t, name, dtype, shape, dev)
+    return t.data_ptr()
+
+
+def _pages(page_table, n_seq, dev):
+    """The page table's address and columns."""
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise InvalidArg("page_table: expected a torch.Tensor [n_seq, max_pages]")
+    rows, cols = page_table.shape
+    if rows < n_seq:
+        raise InvalidArg(f"page_table: shape {(rows, cols)}")
+    return _table(page_table, "page_table", torch.int32, (rows, cols), dev), cols
 
 
 def _float_rows(t, name):
@@ -763,26 +782,28 @@ def _float_rows(t, name):
 def rope_apply(dev: Device, plan: RopePlan, q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor,
                q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
     """q [n, Hq, D] and k [n, Hkv, D] (f32 / f16 / bf16, D contiguous, any other strides) rotated at
-    positions pos int32 [n], into q_out and k_out: new contiguous tensors by default, or q and k themselves for
-    a rotation in place.  Returns (q_out, k_out)."""
-    code, td = _float_rows(q, "q"), dev.torch_device
-    n, hq, d = q.shape
-    qp = _rows(q, "q", q.dtype, q.shape, td)
+    positions pos int32 [n], into q_out and k_out: new tensors (torch.empty_like's) by default, or q and k
+    themselves for a rotation in place.  Returns (q_out, k_out)."""
+    code, td, dt, shape = _float_rows(q, "q"), dev.torch_device, q.dtype, q.shape
+    n, hq, d = shape
+    qp = _rows(q, "q", dt, shape, td)
     if q_out is None:
-        q_out = torch.empty((n, hq, d), dtype=q.dtype, device=td)
-    qo = _rows(q_out, "q_out", q.dtype, q.shape, td)
+        q_out = torch.empty_like(q)
+    qo = _rows(q_out, "q_out", dt, shape, td)
     kp = ko = (None, 0, 0)
     hkv = 0
     if k is not None:
         _float_rows(k, "k")
         hkv = k.shape[1]
-        kp = _rows(k, "k", q.dtype, (n, hkv, d), td)
+        shape = (n, hkv, d)
+        kp = _rows(k, "k", dt, shape, td)
         if k_out is None:
-            k_out = torch.empty((n, hkv, d), dtype=q.dtype, device=td)
-        ko = _rows(k_out, "k_out", q.dtype, (n, hkv, d), td)
-    _need(pos, "pos", torch.int32, (n,), td)
-    dev.check(dev.lib.pi_rope_apply(dev.h, plan.p, code, n, d, pos.data_ptr(), *qp, hq, *qo, *kp, hkv, *ko,
-                                    dev.stream()))
+            k_out = torch.empty_like(k)
+        ko = _rows(k_out, "k_out", dt, shape, td)
+    rc = dev.lib.pi_rope_apply(dev.h, plan.p, code, n, d, _table(pos, "pos", torch.int32, (n,), td), *qp, hq, *qo, *kp, hkv,
+                               *ko, dev.stream())
+    if rc:
+        dev.check(rc)
     return q_out, k_out
 
 
@@ -794,6 +815,7 @@ class Q4Pool:
                  page_tokens: int = PAGE_TOKENS):
         self.p = None
         self.dev = dev
+        self._ws_bytes = {}
         self.n_pages, self.n_kv_heads, self.head_dim = n_pages, n_kv_heads, head_dim
         p = ctypes.c_void_p()
         dev.check(dev.lib.pi_q4_pool_create(dev.h, n_pages, page_tokens, n_kv_heads, head_dim,
@@ -828,38 +850,32 @@ class Q4Pool:
         sequence stay uninitialised)."""
         d, td = self.dev, self.dev.torch_device
         code = _float_rows(k, "k")
-        n, hkv, dh = k.shape
-        shape = (n, self.n_kv_heads, self.head_dim)
-        kp = _rows(k, "k", k.dtype, shape, td)
-        vp = _rows(v, "v", k.dtype, shape, td)
-        if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
-            raise InvalidArg("page_table: expected a torch.Tensor [n_seq, max_pages]")
+        dt, n, dh = k.dtype, k.shape[0], self.head_dim
+        shape = (n, self.n_kv_heads, dh)
+        kp = _rows(k, "k", dt, shape, td)
+        vp = _rows(v, "v", dt, shape, td)
         n_seq = start_pos.shape[0] if isinstance(start_pos, torch.Tensor) and start_pos.dim() == 1 else -1
-        _need(page_table, "page_table", torch.int32, dev=td)
-        _need(start_pos, "start_pos", torch.int32, (n_seq,), td)
-        if page_table.shape[0] < n_seq:
-            raise InvalidArg(f"page_table: shape {tuple(page_table.shape)}")
-        if tok_start is not None:
-            _need(tok_start, "tok_start", torch.int32, (n_seq + 1,), td)
+        pt, cols = _pages(page_table, n_seq, td)
+        sp = _table(start_pos, "start_pos", torch.int32, (n_seq,), td)
+        ts = _table(tok_start, "tok_start", torch.int32, (n_seq + 1,), td)
         qp = qo = (None, 0, 0)
         hq = 0
         if q is not None:
             _float_rows(q, "q")
             hq = q.shape[1]
-            qp = _rows(q, "q", k.dtype, (n, hq, dh), td)
+            qp = _rows(q, "q", dt, (n, hq, dh), td)
             if q_out is None:
-                q_out = torch.empty((n, hq, dh), dtype=q.dtype, device=td)
-            qo = _rows(q_out, "q_out", k.dtype, (n, hq, dh), td)
-        for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
-            if w is not None:
-                _need(w, name, torch.float32, (dh,), td)
-        kv = torch.empty((2,) + shape, dtype=torch.float16, device=td) if values else None
-        at = kv.data_ptr() if values else None
-        d.check(d.lib.pi_q4_append(d.h, self.p, None if plan is None else plan.p, code, n, _vp(tok_start),
-                                   start_pos.data_ptr(), n_seq, page_table.data_ptr(), page_table.shape[1],
-                                   *qp, hq, *qo, *kp, *vp, _vp(q_norm_w), _vp(k_norm_w), float(eps), at,
-                                   at + kv[0].numel() * 2 if values else None, d.stream()))
-        return (q_out, kv[0], kv[1]) if values else q_out
+                q_out = torch.empty((n, hq, dh), dtype=dt, device=td)
+            qo = _rows(q_out, "q_out", dt, (n, hq, dh), td)
+        qw = _table(q_norm_w, "q_norm_w", torch.float32, (dh,), td)
+        kw = _table(k_norm_w, "k_norm_w", torch.float32, (dh,), td)
+        k_val = torch.empty(shape, dtype=torch.float16, device=td) if values else None
+        v_val = torch.empty(shape, dtype=torch.float16, device=td) if values else None
+        rc = d.lib.pi_q4_append(d.h, self.p, None if plan is None else plan.p, code, n, ts, sp, n_seq, pt, cols, *qp, hq, *qo,
+                                *kp, *vp, qw, kw, float(eps), _vp(k_val), _vp(v_val), d.stream())
+        if rc:
+            d.check(rc)
+        return (q_out, k_val, v_val) if values else q_out
 
     def _record_shapes(self, n):
         hk, d = self.n_kv_heads, self.head_dim
@@ -892,40 +908,43 @@ class Q4Pool:
                                   *(t.data_ptr() for t in args), d.stream()))
 
 
-def _q4_attn(entry, dev, q, pool, page_table, n_seq, tok_start, pos, max_tok, max_ctx, gqa_mode, scale, gate, out,
-             ws):
-    code, td = _float_rows(q, "q"), dev.torch_device
-    _need(q, "q", dev=td)
-    n, hq, dh = q.shape
+def _q4_attn(entry, dev, q, pool, page_table, n_seq, ts, pos, max_tok, max_ctx, gqa_mode, scale, gate, out, ws):
+    code, td, dt, shape = _float_rows(q, "q"), dev.torch_device, q.dtype, q.shape
+    n, hq, dh = shape
+    qp = _table(q, "q", dt, shape, td)
     if dh != pool.head_dim:
         raise InvalidArg(f"q head_dim {dh} != pool head_dim {pool.head_dim}")
-    _need(page_table, "page_table", torch.int32, dev=td)
-    if page_table.dim() != 2 or page_table.shape[0] < n_seq:
-        raise InvalidArg(f"page_table: shape {tuple(page_table.shape)}")
-    if gate is not None:
-        _need(gate, "gate", q.dtype, q.shape, td)
+    pt, max_pages = _pages(page_table, n_seq, td)
+    gp = _table(gate, "gate", dt, shape, td)
     if out is None:
         out = torch.empty_like(q)
-    _need(out, "out", q.dtype, q.shape, td)
-    max_pages, max_ctx = page_table.shape[1], 0 if max_ctx is None else int(max_ctx)
-    need = ctypes.c_size_t()
-    dev.check(dev.lib.pi_q4_attn_ws_bytes(dev.h, pool.p, code, n, n_seq, max_tok, max_pages, max_ctx, hq, gqa_mode,
-                                          ctypes.byref(need)))
-    if ws is None:  # torch's allocator keeps it with the stream, and with the graph under capture
-        ws = torch.empty(need.value, dtype=torch.uint8, device=td) if need.value else None
-    elif not isinstance(ws, torch.Tensor) or ws.device != td or not ws.is_contiguous():
-        raise InvalidArg("ws: expected a contiguous torch.Tensor on the device")
+    op = _table(out, "out", dt, shape, td)
+    max_ctx = 0 if max_ctx is None else int(max_ctx)
+    key = (code, n, n_seq, max_tok, max_pages, max_ctx, hq, gqa_mode)
+    need = pool._ws_bytes.get(key)  # a function of the sizes alone
+    if need is None:
+        size = ctypes.c_size_t()
+        dev.check(dev.lib.pi_q4_attn_ws_bytes(dev.h, pool.p, *key, ctypes.byref(size)))
+        if len(pool._ws_bytes) >= 4096:
+            pool._ws_bytes.clear()
+        need = pool._ws_bytes[key] = size.value
+    wp, wn = None, 0
+    if ws is not None:
+        if not isinstance(ws, torch.Tensor) or ws.device != td or not ws.is_contiguous():
+            raise InvalidArg("ws: expected a contiguous torch.Tensor on the device")
+        wp, wn = ws.data_ptr(), ws.numel() * ws.element_size()
+    elif need:  # torch's allocator keeps it with the stream, and with the graph under capture
+        ws = torch.empty(need, dtype=torch.uint8, device=td)
+        wp, wn = ws.data_ptr(), need
     if scale is None:
         scale = 1.0 / math.sqrt(dh)
-    ws_ptr, ws_bytes = (None, 0) if ws is None else (ws.data_ptr(), ws.numel() * ws.element_size())
-    if tok_start is None:
-        rc = entry(dev.h, pool.p, q.data_ptr(), code, page_table.data_ptr(), max_pages, max_ctx, pos.data_ptr(), n, hq,
-                   gqa_mode, float(scale), _vp(gate), out.data_ptr(), ws_ptr, ws_bytes, dev.stream())
+    if ts is None:
+        rc = entry(dev.h, pool.p, qp, code, pt, max_pages, max_ctx, pos, n, hq, gqa_mode, scale, gp, op, wp, wn, dev.stream())
     else:
-        rc = entry(dev.h, pool.p, q.data_ptr(), code, n, tok_start.data_ptr(), pos.data_ptr(), n_seq, max_tok,
-                   page_table.data_ptr(), max_pages, max_ctx, hq, gqa_mode, float(scale), _vp(gate), out.data_ptr(),
-                   ws_ptr, ws_bytes, dev.stream())
-    dev.check(rc)
+        rc = entry(dev.h, pool.p, qp, code, n, ts, pos, n_seq, max_tok, pt, max_pages, max_ctx, hq, gqa_mode, scale, gp, op, wp,
+                   wn, dev.stream())
+    if rc:
+        dev.check(rc)
     return out
 
 
@@ -937,8 +956,10 @@ def q4_attn_decode(dev: Device, q: torch.Tensor, pool: Q4Pool, page_table: torch
     max_ctx: a bound of ctx_len (default: the table's row).  ws: a workspace of the caller's; by default
     the call takes one from torch's allocator."""
     b = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else 0
-    _need(ctx_len, "ctx_len", torch.int32, (b,), dev.torch_device)
-    return _q4_attn(dev.lib.pi_q4_attn_decode, dev, q, pool, page_table, b, None, ctx_len, 1, max_ctx, gqa_mode, scale,
+    if ctx_len is None:
+        raise InvalidArg("ctx_len: expected a torch.Tensor")
+    cl = _table(ctx_len, "ctx_len", torch.int32, (b,), dev.torch_device)
+    return _q4_attn(dev.lib.pi_q4_attn_decode, dev, q, pool, page_table, b, None, cl, 1, max_ctx, gqa_mode, scale,
                     gate, out, ws)
 
 
@@ -951,8 +972,10 @@ def q4_attn_prefill(dev: Device, q: torch.Tensor, pool: Q4Pool, page_table: torc
     at positions start_pos[s] ... (their keys appended first) -> out like q.  max_tok: no sequence has more
     rows (default: n).  Rows of no sequence are left as they were in `out`."""
     n_seq = start_pos.shape[0] if isinstance(start_pos, torch.Tensor) and start_pos.dim() == 1 else -1
-    _need(start_pos, "start_pos", torch.int32, (n_seq,), dev.torch_device)
-    _need(tok_start, "tok_start", torch.int32, (n_seq + 1,), dev.torch_device)
     n = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else 0
-    return _q4_attn(dev.lib.pi_q4_attn_prefill, dev, q, pool, page_table, n_seq, tok_start, start_pos,
+    if start_pos is None or tok_start is None:
+        raise InvalidArg("start_pos and tok_start: expected torch.Tensors")
+    sp = _table(start_pos, "start_pos", torch.int32, (n_seq,), dev.torch_device)
+    ts = _table(tok_start, "tok_start", torch.int32, (n_seq + 1,), dev.torch_device)
+    return _q4_attn(dev.lib.pi_q4_attn_prefill, dev, q, pool, page_table, n_seq, ts, sp,
                     n if max_tok is None else int(max_tok), max_ctx, gqa_mode, scale, gate, out, ws)
