@@ -128,8 +128,8 @@ struct Chunks {
     int a, b;
     bool turn;  // halves: the two chunks rotate together
 };
-template <bool VEC>
-__device__ __forceinline__ Chunks chunks_of(int c, int D, int half, int layout) {
+template <bool VEC, int D>
+__device__ __forceinline__ Chunks chunks_of(int c, int half, int layout) {
     if (!VEC) return {8 * c, 8 * c, false};
     if (layout != 1 || half == 0) return {8 * c, 8 * c + D / 2, false};
     if (8 * c < half) return {8 * c, 8 * c + half, true};
@@ -171,11 +171,11 @@ struct Weights {
     }
 };
 
-// Norm and rotation of a lane's channels; lpr lanes hold the row.  cs: cos and sin of the token's pairs.  u, v: the chunks
+// Norm and rotation of a lane's channels.  cs: cos and sin of the token's pairs.  u, v: the chunks
 // (v: VEC only).
-template <typename T, typename R, typename R2, bool VEC>
-__device__ __forceinline__ void norm_rotate(const Raw<T, VEC>& raw, const Chunks& ch, int D, int lpr, const Weights& w, float eps, int half,
-                                            int layout, const R2* cs, R* u, R* v) {
+template <typename T, typename R, typename R2, bool VEC, int D>
+__device__ __forceinline__ void norm_rotate(const Raw<T, VEC>& raw, const Chunks& ch, const Weights& w, float eps, int half, int layout,
+                                            const R2* cs, R* u, R* v) {
     typedef Real<R> F;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -186,7 +186,8 @@ __device__ __forceinline__ void norm_rotate(const Raw<T, VEC>& raw, const Chunks
         R ss = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss += VEC ? u[e] * u[e] + v[e] * v[e] : u[e] * u[e];
-        for (int m = 1; m < lpr; m <<= 1) ss += shfl_xor(ss, m);
+#pragma unroll
+        for (int m = 1; m < D / (VEC ? 16 : 8); m <<= 1) ss += shfl_xor(ss, m);
         const R rs = F::inv_sqrt(ss / (R)D + (R)eps);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -284,19 +285,20 @@ __device__ __forceinline__ void store8(T* out, const float* y) {
 }
 
 // A lane's channels of a query row: normed, rotated, written in the rows' type.
-template <typename T, bool VEC>
+template <typename T, bool VEC, int D>
 __device__ __forceinline__ void put_q(const Q4AppendArgs& a, const Raw<T, VEC>& raw, const Weights& w, int row, int h, const Chunks& ch,
-                                      int lpr, const float2* cs) {
+                                      const float2* cs) {
     float u[8], v[8];
-    norm_rotate<T, float, float2, VEC>(raw, ch, a.g.head_dim, lpr, w, a.eps, a.plan.half, a.plan.layout, cs, u, v);
+    norm_rotate<T, float, float2, VEC, D>(raw, ch, w, a.eps, a.plan.half, a.plan.layout, cs, u, v);
     T* out = static_cast<T*>(a.q_out.p) + row * a.q_out.tok + h * a.q_out.head;
     store8<T, VEC>(out + ch.a, u);
     if (VEC) store8<T, VEC>(out + ch.b, v);
 }
 
 // A chunk's codes w and scale s to its page, and its values to where the caller wants them.
+template <int D>
 __device__ __forceinline__ void put_codes(const Q4AppendArgs& a, uint32_t w, float s, bool is_v, int row, int kh, int d0, const Place& pl) {
-    const int D = a.g.head_dim, hkv = a.g.n_kv_heads, c = d0 >> 3;
+    const int hkv = a.g.n_kv_heads, c = d0 >> 3;
     uint16_t* val = is_v ? a.v_val : a.k_val;
     if (val) {
         typedef f16 h8 __attribute__((ext_vector_type(8)));
@@ -329,14 +331,14 @@ __device__ __forceinline__ void put_codes(const Q4AppendArgs& a, uint32_t w, flo
 }
 
 // A lane's channels of a key or value row: normed and rotated (keys), quantised, stored.
-template <typename T, bool VEC>
+template <typename T, bool VEC, int D>
 __device__ __forceinline__ void put_kv(const Q4AppendArgs& a, const Raw<T, VEC>& raw, const Weights& nw, bool is_v, int row, int kh,
-                                       const Chunks& ch, int lpr, const Place& pl, const double2* cs) {
+                                       const Chunks& ch, const Place& pl, const double2* cs) {
     float s0, s1 = 0.f;
     uint32_t w0, w1 = 0;
     if (!is_v) {
         double u[8], v[8];
-        norm_rotate<T, double, double2, VEC>(raw, ch, a.g.head_dim, lpr, nw, a.eps, a.plan.half, a.plan.layout, cs, u, v);
+        norm_rotate<T, double, double2, VEC, D>(raw, ch, nw, a.eps, a.plan.half, a.plan.layout, cs, u, v);
         w0 = quantise8<double>(u, &s0);
         if (VEC) w1 = quantise8<double>(v, &s1);
     } else {
@@ -350,38 +352,48 @@ __device__ __forceinline__ void put_kv(const Q4AppendArgs& a, const Raw<T, VEC>&
         w0 = quantise8<R>(u, &s0);
         if (VEC) w1 = quantise8<R>(v, &s1);
     }
-    put_codes(a, w0, s0, is_v, row, kh, ch.a, pl);
-    if (VEC) put_codes(a, w1, s1, is_v, row, kh, ch.b, pl);
+    put_codes<D>(a, w0, s0, is_v, row, kh, ch.a, pl);
+    if (VEC) put_codes<D>(a, w1, s1, is_v, row, kh, ch.b, pl);
 }
 
 // Workgroups 0 .. kv_wgs - 1 take the keys and values of `toks` tokens each (f64 angles, quantiser), the others the
 // queries of `toks` tokens (f32): in one launch, so that the heavier arithmetic runs beside the larger share
 // of the bytes.  blockIdx.y: a share of the tokens' rows.  A workgroup's first rows are requested before it looks
 // up its tokens' places and computes their angles.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4) void q4_append_kernel(Q4AppendArgs a, int toks, int kv_wgs) {
+template <typename T, bool VEC, int D>
+__global__ __launch_bounds__(kThreads, 3) void q4_append_kernel(Q4AppendArgs a, int toks, int kv_wgs) {
     __shared__ double2 s_cs[kTable];
     __shared__ Place s_place[kMaxToks];
-    const int tid = threadIdx.x, D = a.g.head_dim, half = a.plan.half;
+    const int tid = threadIdx.x, half = a.plan.half;
     const bool kv = (int)blockIdx.x < kv_wgs;
     const int row0 = (kv ? blockIdx.x : blockIdx.x - kv_wgs) * toks, n = min(toks, a.n_rows - row0);
-    const int hkv = a.g.n_kv_heads, heads = kv ? 2 * hkv : a.q.n;
-    const int lpr = D / (VEC ? 16 : 8), rpi = kThreads / lpr;  // lanes a row, rows at a time
+    const int hkv = a.g.n_kv_heads, heads = kv ? hkv : a.q.n, n_keys = kv ? n * hkv : 0;
+    constexpr int lpr = D / (VEC ? 16 : 8), rpi = kThreads / lpr;  // lanes a row, rows at a time
     const int rl = tid / lpr;
-    const Chunks ch = chunks_of<VEC>(tid - rl * lpr, D, half, a.plan.layout);
+    const Chunks ch = chunks_of<VEC, D>(tid - rl * lpr, half, a.plan.layout);
     const int step = gridDim.y * rpi;
-    int u = blockIdx.y * rpi + rl, t = u / heads, h = u - t * heads;
+    // Row u: all tokens' key rows, then all their value rows (the key rows' f64 work then falls to all wavefronts alike);
+    // or the query rows.  t, h: its token and head, is_v: a value row.
+    int u = blockIdx.y * rpi + rl, t, h;
+    bool is_v;
+    auto place = [&] {
+        is_v = kv && u >= n_keys;
+        const int r = is_v ? u - n_keys : u;
+        t = r / heads;
+        h = r - t * heads;
+    };
+    place();
     const T* const p0 = static_cast<const T*>(kv ? a.k.p : a.q.p);
     const T* const p1 = static_cast<const T*>(a.v.p);
     const int64_t tok0 = kv ? a.k.tok : a.q.tok, head0 = kv ? a.k.head : a.q.head, tok1 = a.v.tok, head1 = a.v.head;
-    auto load = [&](Raw<T, VEC>& r, int tt, int hh) {
-        if (tt >= n) return;
-        const bool is_v = kv && hh >= hkv;
-        const T* row = is_v ? p1 + (row0 + tt) * tok1 + (hh - hkv) * head1 : p0 + (row0 + tt) * tok0 + hh * head0;
-        r.load(row, ch, is_v ? 0 : half, a.plan.layout);
-    };
+    const int rows = kv ? 2 * n_keys : n * heads;
     Raw<T, VEC> raw;
-    load(raw, t, h);
+    auto load = [&] {
+        if (u >= rows) return;
+        const T* row = is_v ? p1 + (row0 + t) * tok1 + h * head1 : p0 + (row0 + t) * tok0 + h * head0;
+        raw.load(row, ch, is_v ? 0 : half, a.plan.layout);
+    };
+    load();
     Weights w;
     w.template load<VEC>(kv ? a.k_norm : a.q_norm, ch, half, a.plan.layout);
     if (tid < 64) find_places(a, row0, n, s_place, kv);
@@ -407,25 +419,25 @@ __global__ __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : 4) void q4_append_ke
         }
     }
     __syncthreads();
-    while (t < n) {
+    while (u < rows) {
         const Raw<T, VEC> now = raw;
         const int tn = t, hn = h;
+        const bool vn = is_v;
         u += step;
-        t = u / heads;
-        h = u - t * heads;
-        load(raw, t, h);
+        place();
+        load();
         const Place pl = s_place[tn];
         if (pl.pos < 0) continue;  // a row of no sequence; uniform over a row's lanes
         if (kv)
-            put_kv<T, VEC>(a, now, w, hn >= hkv, row0 + tn, hn >= hkv ? hn - hkv : hn, ch, lpr, pl, s_cs + tn * half);
+            put_kv<T, VEC, D>(a, now, w, vn, row0 + tn, hn, ch, pl, s_cs + tn * half);
         else
-            put_q<T, VEC>(a, now, w, row0 + tn, hn, ch, lpr, reinterpret_cast<const float2*>(s_cs) + tn * half);
+            put_q<T, VEC, D>(a, now, w, row0 + tn, hn, ch, reinterpret_cast<const float2*>(s_cs) + tn * half);
     }
 }
 
-template <typename T>
-hipError_t launch_append_t(const Q4AppendArgs& a, hipStream_t s) {
-    const int e = (int)sizeof(T), D = a.g.head_dim;
+template <typename T, int D>
+hipError_t launch_append_d(const Q4AppendArgs& a, hipStream_t s) {
+    const int e = (int)sizeof(T);
     const int half = a.plan.half;
     bool vec = a.plan.layout == 1 && half ? half % 32 == 0 && (D - 2 * half) % 64 == 0 : half % 4 == 0;
     for (const HeadRows* r : {&a.q, &a.q_out, &a.k, &a.v})
@@ -439,10 +451,19 @@ hipError_t launch_append_t(const Q4AppendArgs& a, hipStream_t s) {
     const int y = all * blocks <= 2048 ? std::min(blocks, 65535) : 1;
     const dim3 grid((unsigned)all, y);
     if (vec)
-        hipLaunchKernelGGL((q4_append_kernel<T, true>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
+        hipLaunchKernelGGL((q4_append_kernel<T, true, D>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
     else
-        hipLaunchKernelGGL((q4_append_kernel<T, false>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
+        hipLaunchKernelGGL((q4_append_kernel<T, false, D>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
     return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_append_t(const Q4AppendArgs& a, hipStream_t s) {
+    switch (a.g.head_dim) {
+        case 64: return launch_append_d<T, 64>(a, s);
+        case 128: return launch_append_d<T, 128>(a, s);
+        default: return launch_append_d<T, 256>(a, s);
+    }
 }
 
 // One byte of codes a thread (two channels of a token), the group's scale with its first.
