@@ -32,7 +32,7 @@ constexpr int kWaves = sched::kWaves;
 constexpr int kThreads = 64 * kWaves;
 constexpr float kLazy = 8.0f;     // log2 headroom before the running max moves
 constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
-constexpr int kStage = 2048;      // most floats a wavefront stages at a time for the merge in LDS
+constexpr int kStage = 1024;      // most floats a wavefront stages at a time for the merge in LDS
 constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
 constexpr long long kWholeBytes = 96 << 10;
 constexpr int kAlign = 8;         // grid workgroups a segment from which segments are cut into pieces of their own
@@ -46,7 +46,8 @@ struct Ring {
     static constexpr int kWide = kBytes / 1024, kNarrow = (kBytes % 1024 + 255) / 256;  // 16- and 4-byte loads of 64 lanes
     static constexpr int kSlot = kWide * 1024 + kNarrow * 256;  // D 64: the last load reads half a load past the block
     static constexpr int kLoads = kWide + kNarrow;
-    static constexpr int kPages = D == 256 ? 4 : 8;             // slots: a pair at work, the others in flight
+    // Slots: a pair at work, the others in flight.  The LDS then holds two (D 256) or three workgroups a CU, as the registers do.
+    static constexpr int kPages = D == 256 ? 4 : D == 128 ? 5 : 8;
 };
 
 static_assert(kStage * 4 <= Ring<64>::kPages * Ring<64>::kSlot && kStage * 4 <= Ring<256>::kPages * Ring<256>::kSlot, "O is staged in the rings");
@@ -178,29 +179,30 @@ struct Acc {
 
 // Two pages: scores, softmax, values.  lim[cb]: keys below it are seen by the lane's row; tok0[u]: first token
 // of page u; edge: some row's limit may fall inside (then tokens are compared).
-template <typename T, int D, int NCB>
+// N: the row blocks that hold rows, of NCB.
+template <typename T, int D, int NCB, int N>
 __device__ __forceinline__ void process(Acc<D, NCB>& acc, const Page<D>* pg, const Query<T, D>* q, const float* back, const int* lim,
                                         const int* tok0, bool edge, int grp, const Q4Magic& mg) {
     constexpr int NJ = D / kQ4Group, PREC = Query<T, D>::PREC;
-    f32x4 s[2][NCB];
+    f32x4 s[2][N];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) s[u][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int cb = 0; cb < N; ++cb) s[u][cb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const f16x2 sc = __builtin_bit_cast(f16x2, pg[u].ks.w[j / 2]);
             const f16x8 kf = deq_k(pg[u].k.w[j], sc[j & 1], mg);
 #pragma unroll
-            for (int cb = 0; cb < NCB; ++cb)
+            for (int cb = 0; cb < N; ++cb)
 #pragma unroll
                 for (int h = 0; h < PREC; ++h)
                     s[u][cb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[cb].r[h][j], s[u][cb], 0, 0, 0);
         }
     }
-    f16x8 pb[NCB][PREC];
+    f16x8 pb[N][PREC];
 #pragma unroll
-    for (int cb = 0; cb < NCB; ++cb) {
+    for (int cb = 0; cb < N; ++cb) {
         float mx = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -253,7 +255,7 @@ __device__ __forceinline__ void process(Acc<D, NCB>& acc, const Page<D>* pg, con
         const f16x8 hi = join4(deq_pair(w0, a0, oa0, mg), deq_pair(w0 >> 8, b0, ob0, mg), deq_pair(w1, a1, oa1, mg),
                                deq_pair(w1 >> 8, b1, ob1, mg));
 #pragma unroll
-        for (int cb = 0; cb < NCB; ++cb)
+        for (int cb = 0; cb < N; ++cb)
 #pragma unroll
             for (int h = 0; h < PREC; ++h) {
                 acc.o[cb][2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pb[cb][h], acc.o[cb][2 * j], 0, 0, 0);
@@ -378,6 +380,8 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
         float back[NCB];
         int lim[NCB];
         bool have_q = false;
+        // 16-row blocks with rows of this sequence (a ragged batch's shorter chunks fill fewer)
+        const int live = __builtin_amdgcn_readfirstlane(min(NCB, (rw.n * a.group - row0 + 15) / 16));
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
 #pragma unroll
@@ -385,74 +389,81 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
             acc.m[cb] = -1e30f;
             acc.l[cb] = 0.f;
         }
-        for (int sub = run.pg0; sub < run.pg1; sub += sched::kSubPages) {
-            int first, n_my;
-            sched::sub_pages(sub, run.pg1, wave, &first, &n_my);
-            // A page id outside the pool holds no tokens: page 0 is read in its place, all of it masked.
-            const int pid_raw = lane < n_my ? pt[first + kWaves * lane] : 0;
-            const bool bad = !sched::page_ok(pid_raw, a.g.n_pages);
-            const int pid_v = bad ? 0 : pid_raw;
-            const uint64_t bad_pages = __ballot(bad);
-            constexpr int kNone = 0x7fffffc0;  // a page whose tokens are past every limit
-            auto issue = [&](int j) {  // page j of the wavefront's into its slot
-                const int pid = __builtin_amdgcn_readlane(pid_v, j);
-                load_block<D>(a.g.base + ((size_t)pid * n_kv + kvh) * blk_bytes, ring_at + (j % R::kPages) * R::kSlot, lane16, lane4);
-            };
-            for (int j = 0; j < min(n_my, R::kPages); ++j) issue(j);
-            if (!have_q) {  // the rows, while the first pages are on their way
-                have_q = true;
+        auto walk = [&](auto blocks) {  // the run's pages for the first N row blocks
+            constexpr int N = decltype(blocks)::value;
+            for (int sub = run.pg0; sub < run.pg1; sub += sched::kSubPages) {
+                int first, n_my;
+                sched::sub_pages(sub, run.pg1, wave, &first, &n_my);
+                // A page id outside the pool holds no tokens: page 0 is read in its place, all of it masked.
+                const int pid_raw = lane < n_my ? pt[first + kWaves * lane] : 0;
+                const bool bad = !sched::page_ok(pid_raw, a.g.n_pages);
+                const int pid_v = bad ? 0 : pid_raw;
+                const uint64_t bad_pages = __ballot(bad);
+                constexpr int kNone = 0x7fffffc0;  // a page whose tokens are past every limit
+                auto issue = [&](int j) {  // page j of the wavefront's into its slot
+                    const int pid = __builtin_amdgcn_readlane(pid_v, j);
+                    load_block<D>(a.g.base + ((size_t)pid * n_kv + kvh) * blk_bytes, ring_at + (j % R::kPages) * R::kSlot, lane16, lane4);
+                };
+                for (int j = 0; j < min(n_my, R::kPages); ++j) issue(j);
+                if (!have_q) {  // the rows, while the first pages are on their way
+                    have_q = true;
 #pragma unroll
-                for (int cb = 0; cb < NCB; ++cb) {
-                    const int r = cb * 16 + col;
-                    const long long off = r < a.cols ? row_offset(a, rw, kvh, row0 + r, D) : -1;
-                    back[cb] = q[cb].load(static_cast<const T*>(a.q), off, grp, a.scale);
-                    lim[cb] = min(rw.start + (row0 + r) / a.group + 1, rw.len);
+                    for (int cb = 0; cb < NCB; ++cb) {
+                        const int r = cb * 16 + col;
+                        const long long off = r < a.cols ? row_offset(a, rw, kvh, row0 + r, D) : -1;
+                        back[cb] = q[cb].load(static_cast<const T*>(a.q), off, grp, a.scale);
+                        lim[cb] = min(rw.start + (row0 + r) / a.group + 1, rw.len);
+                    }
+                }
+                // pages 2 i and 2 i + 1 have landed; the younger ones may still be under way
+                auto landed = [&](int i) {
+                    constexpr int kAhead = R::kPages - 2;
+                    const int ahead = n_my - 2 * i - 2;  // pages behind the pair
+                    if (kAhead >= 6 && ahead >= 6)
+                        wait_loads<(kAhead >= 6 ? 6 : 0) * R::kLoads>();
+                    else if (kAhead >= 4 && ahead >= 4)
+                        wait_loads<(kAhead >= 4 ? 4 : 0) * R::kLoads>();
+                    else if (ahead >= 2)
+                        wait_loads<2 * R::kLoads>();
+                    else
+                        wait_loads<0>();
+                };
+                auto fetch = [&](Page<D>* pg, int i) {  // the pair to registers; a second page that does not exist: the first, masked
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) pg[u].load(ring + ((2 * i + u < n_my ? 2 * i + u : 2 * i) % R::kPages) * R::kSlot, lane);
+                };
+                auto run_pair = [&](const Page<D>* pg, int i) {
+                    int tok0[2];
+                    bool edge = false;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int j = 2 * i + u;
+                        const int t = (first + kWaves * j) * sched::kPage;
+                        const bool on = j < n_my && !((bad_pages >> j) & 1);
+                        tok0[u] = on ? t : kNone;
+                        edge = edge || !on || t + sched::kPage > first_lim;
+                    }
+                    process<T, D, NCB, N>(acc, pg, q, back, lim, tok0, edge, grp, mg);
+                };
+                auto refill = [&](int i) {  // the pair's slots, once it is in registers
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        if (2 * i + u + R::kPages < n_my) issue(2 * i + u + R::kPages);
+                };
+                const int n_iter = (n_my + 1) / 2;
+                for (int i = 0; i < n_iter; ++i) {
+                    Page<D> x[2];
+                    landed(i);
+                    fetch(x, i);
+                    run_pair(x, i);
+                    refill(i);
                 }
             }
-            // pages 2 i and 2 i + 1 have landed; the younger ones may still be under way
-            auto landed = [&](int i) {
-                constexpr int kAhead = R::kPages - 2;
-                const int ahead = n_my - 2 * i - 2;  // pages behind the pair
-                if (kAhead >= 6 && ahead >= 6)
-                    wait_loads<(kAhead >= 6 ? 6 : 0) * R::kLoads>();
-                else if (kAhead >= 4 && ahead >= 4)
-                    wait_loads<(kAhead >= 4 ? 4 : 0) * R::kLoads>();
-                else if (ahead >= 2)
-                    wait_loads<2 * R::kLoads>();
-                else
-                    wait_loads<0>();
-            };
-            auto fetch = [&](Page<D>* pg, int i) {  // the pair to registers; a second page that does not exist: the first, masked
-#pragma unroll
-                for (int u = 0; u < 2; ++u) pg[u].load(ring + ((2 * i + u < n_my ? 2 * i + u : 2 * i) % R::kPages) * R::kSlot, lane);
-            };
-            auto run_pair = [&](const Page<D>* pg, int i) {
-                int tok0[2];
-                bool edge = false;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int j = 2 * i + u;
-                    const int t = (first + kWaves * j) * sched::kPage;
-                    const bool on = j < n_my && !((bad_pages >> j) & 1);
-                    tok0[u] = on ? t : kNone;
-                    edge = edge || !on || t + sched::kPage > first_lim;
-                }
-                process<T, D, NCB>(acc, pg, q, back, lim, tok0, edge, grp, mg);
-            };
-            auto refill = [&](int i) {  // the pair's slots, once it is in registers
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    if (2 * i + u + R::kPages < n_my) issue(2 * i + u + R::kPages);
-            };
-            const int n_iter = (n_my + 1) / 2;
-            for (int i = 0; i < n_iter; ++i) {
-                Page<D> x[2];
-                landed(i);
-                fetch(x, i);
-                run_pair(x, i);
-                refill(i);
-            }
-        }
+        };
+        if (NCB == 2 && D <= 128 && live == 1)  // (a copy of the loop; in one loop the accumulators would be copied)
+            walk(std::integral_constant<int, 1>{});
+        else
+            walk(std::integral_constant<int, NCB>{});
         // ---- the 4 wavefronts' shares meet in LDS, `stage` floats of rows at a time ----
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
@@ -465,7 +476,8 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
         }
         const size_t slot = (size_t)sched::run_slot(cur == run.seg0, b, sidx, n_seg, a.batch, blockIdx.x);
         __syncthreads();  // (the rings are read no more, either)
-        if (tid < a.cols) {  // each wavefront's weight, and the row's max and sum
+        const int rows = min(a.cols, rw.n * a.group - row0);  // of the block that exist in this sequence
+        if (tid < rows) {  // each wavefront's weight, and the row's max and sum
             float M = s_m[0][tid], lsum = 0.f;
 #pragma unroll
             for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][tid]);
@@ -486,7 +498,7 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
         for (int cb = 0; cb < NCB; ++cb) {
             for (int c0 = 0; c0 < 16; c0 += per) {
                 const int r0 = 16 * cb + c0;  // rows r0 .. r0 + per - 1 of the block
-                if (r0 >= a.cols) break;
+                if (r0 >= rows) break;
                 if (col >= c0 && col < c0 + per) {
 #pragma unroll
                     for (int t = 0; t < D / 16; ++t)
@@ -495,7 +507,7 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
                 __syncthreads();
                 for (int idx = 4 * tid; idx < per * D; idx += 4 * kThreads) {
                     const int c = idx / D, d = idx - c * D, r = r0 + c;
-                    if (r >= a.cols) break;
+                    if (r >= rows) break;
                     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int w = 0; w < kWaves; ++w) o += s_m[w][r] * *reinterpret_cast<const f32x4*>(&s_o[w * stage + idx]);
@@ -554,7 +566,7 @@ __global__ __launch_bounds__(256) void q4_merge_kernel(Q4AttnArgs a, Q4Ws ws, in
     __syncthreads();
     const int c_lo = e0 / D, c_hi = min(cols - 1, (e0 + 64 * V - 1) / D);
     constexpr int kPre = 4;
-    const bool on = e < GD;
+    const bool on = off >= 0;  // partials of rows that do not exist were not written
     const float* po = ws.o + (on ? e : 0);
     auto part = [&](int r) { return *reinterpret_cast<const VT*>(po + (size_t)s_slot[r] * GD); };
     const VT zero = VT{};
@@ -621,10 +633,15 @@ int vgpr_wgs() {  // resident workgroups a CU by registers alone
     }();
     return n;
 }
+// Row blocks of a wavefront, at most: what fits the registers of one wavefront a SIMD.
+template <typename T>
+constexpr int max_ncb(int d) { return (d == 256 ? 2 : 4) / (sizeof(T) == 4 && d != 64 ? 2 : 1); }
+
 template <typename T>
 int wgs_of(int d, int ncb) {
-    if (d == 256) return ncb == 1 ? vgpr_wgs<T, 256, 1>() : vgpr_wgs<T, 256, 2>();
-    if (d == 128) return ncb == 1 ? vgpr_wgs<T, 128, 1>() : ncb == 2 ? vgpr_wgs<T, 128, 2>() : vgpr_wgs<T, 128, 4>();
+    constexpr int M256 = max_ncb<T>(256), M128 = max_ncb<T>(128);
+    if (d == 256) return ncb == 1 ? vgpr_wgs<T, 256, 1>() : vgpr_wgs<T, 256, M256>();
+    if (d == 128) return ncb == 1 ? vgpr_wgs<T, 128, 1>() : ncb == 2 ? vgpr_wgs<T, 128, 2>() : vgpr_wgs<T, 128, M128>();
     return ncb == 1 ? vgpr_wgs<T, 64, 1>() : ncb == 2 ? vgpr_wgs<T, 64, 2>() : vgpr_wgs<T, 64, 4>();
 }
 
@@ -671,10 +688,13 @@ hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStrea
 
 template <typename T>
 hipError_t launch_d(const Q4AttnArgs& a, const Q4Plan& p, void* ws, hipStream_t s) {
+    constexpr int M256 = max_ncb<T>(256), M128 = max_ncb<T>(128);
     const int d = a.g.head_dim;
-    if (d == 256) return p.ncb == 1 ? launch_t<T, 256, 1>(a, p, ws, s) : launch_t<T, 256, 2>(a, p, ws, s);
+    if (d == 256) return p.ncb == 1 ? launch_t<T, 256, 1>(a, p, ws, s) : launch_t<T, 256, M256>(a, p, ws, s);
     if (d == 128)
-        return p.ncb == 1 ? launch_t<T, 128, 1>(a, p, ws, s) : p.ncb == 2 ? launch_t<T, 128, 2>(a, p, ws, s) : launch_t<T, 128, 4>(a, p, ws, s);
+        return p.ncb == 1   ? launch_t<T, 128, 1>(a, p, ws, s)
+               : p.ncb == 2 ? launch_t<T, 128, 2>(a, p, ws, s)
+                            : launch_t<T, 128, M128>(a, p, ws, s);
     return p.ncb == 1 ? launch_t<T, 64, 1>(a, p, ws, s) : p.ncb == 2 ? launch_t<T, 64, 2>(a, p, ws, s) : launch_t<T, 64, 4>(a, p, ws, s);
 }
 
@@ -701,10 +721,9 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
         p.ws_bytes = p.merge ? (size_t)splits * a.n_rows * a.n_q_heads * (d + 2) * 4 : 0;
         return p;
     }
-    const int most = d == 256 ? 2 : 4;
+    const int most = a.dtype == 0 ? max_ncb<float>(d) : max_ncb<f16>(d);
     const long long blocks = (rows + 15) / 16;
-    p.ncb = blocks >= 3 ? most : (int)blocks;
-    p.ncb = p.ncb == 3 ? 4 : p.ncb;
+    p.ncb = blocks >= most ? most : blocks == 3 ? 4 : (int)blocks;
     a.n_cb = (int)((rows + 16 * p.ncb - 1) / (16 * p.ncb));
     a.cols = (int)std::min<long long>(rows, 16 * p.ncb);
     const int n_seg = n_kv * a.n_cb;
