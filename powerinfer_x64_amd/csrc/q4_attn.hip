@@ -33,6 +33,7 @@ constexpr int kThreads = 64 * kWaves;
 constexpr float kLazy = 8.0f;     // log2 headroom before the running max moves
 constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
 constexpr int kStage = 1024;      // most floats a wavefront stages at a time for the merge in LDS
+constexpr int kMaxSplits = 32;    // key splits of a tiled row block
 constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
 constexpr long long kWholeBytes = 96 << 10;
 constexpr int kAlign = 8;         // grid workgroups a segment from which segments are cut into pieces of their own
@@ -712,7 +713,7 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
         const long long n_blk = (rows + per - 1) / per, wgs = n_blk * n_kv * a.batch;
         p.tiles = true;
         // Few row blocks: their keys are split while that fills idle CUs and each part keeps 4 tiles.
-        long long splits = wgs >= cus ? 1 : std::min<long long>({8, cus / wgs, a.use_pages / 16});
+        long long splits = wgs >= cus ? 1 : std::min<long long>({kMaxSplits, cus / wgs, a.use_pages / 16});
         splits = std::max<long long>(splits, 1);
         p.splits = (int)splits;
         p.n_blk = (int)n_blk;

@@ -452,37 +452,46 @@ __global__ __launch_bounds__(256) void q4_tile_merge_kernel(Q4AttnArgs a, TileAr
     const size_t rows = (size_t)a.n_rows * a.n_q_heads;
     const size_t row = (size_t)blockIdx.x * per + rl;
     if (row >= rows) return;
-    // rows of no sequence, and rows past max_tok, hold no partials
+    // Rows of no sequence, and rows past max_tok, hold no partials: they are read (the
+    // workspace covers them) and not stored. The D / 4 lanes of a row look at as many
+    // sequences at once; one after the other each costs a trip to the L2.
     const int tok = (int)(row / a.n_q_heads);
-    bool mine = false;
-    for (int b0 = 0; b0 < a.batch; ++b0) {
+    bool in_seq = false;
+    for (int b0 = d / 4; b0 < a.batch; b0 += D / 4) {
         const Q4Rows rw = q4_rows(a.tok_start, a.pos, b0, a.n_rows, a.max_tok, a.use_pages);
-        if (tok >= rw.first && tok < rw.first + rw.n) {
-            mine = true;
-            break;
+        in_seq |= tok >= rw.first && tok < rw.first + rw.n;
+    }
+    const int lane = threadIdx.x & 63;
+    const uint64_t lanes = (D == 256 ? ~0ull : (1ull << (D / 4)) - 1) << (lane & ~(D / 4 - 1));
+    const bool mine = (__ballot(in_seq) & lanes) != 0;
+    // four splits' loads in flight at a time, joined against the running maximum
+    float mx = -1e30f, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < ta.splits; s0 += 4) {
+        float mm[4], ll[4];
+        f32x4 oo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = s0 + i < ta.splits;
+            const size_t p = (in ? s0 + i : s0) * rows + row;
+            mm[i] = ta.ml[2 * p];
+            ll[i] = in ? ta.ml[2 * p + 1] : 0.f;
+            oo[i] = *reinterpret_cast<const f32x4*>(ta.o + p * D + d);
+        }
+        const float was = mx;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, mm[i]);
+        const float f = fast_exp2(was - mx);
+        o *= f;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = s0 + i < ta.splits ? fast_exp2(mm[i] - mx) : 0.f;
+            o += w * oo[i];
+            l += w * ll[i];
         }
     }
     if (!mine) return;
-    float mx = -1e30f, l = 0.f;
-    float mm[8], ll[8];
-    f32x4 oo[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        if (s >= ta.splits) break;
-        const size_t p = s * rows + row;
-        mm[s] = ta.ml[2 * p];
-        ll[s] = ta.ml[2 * p + 1];
-        oo[s] = *reinterpret_cast<const f32x4*>(ta.o + p * D + d);
-        mx = fmaxf(mx, mm[s]);
-    }
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        if (s >= ta.splits) break;
-        const float w = fast_exp2(mm[s] - mx);
-        o += w * oo[s];
-        l += w * ll[s];
-    }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     typedef T t4 __attribute__((ext_vector_type(4)));
     t4 y;
