@@ -35,9 +35,9 @@ constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
 constexpr int kStage = 1024;      // most floats a wavefront stages at a time for the merge in LDS
 constexpr int kMaxSplits = 32;    // key splits of a tiled row block
 constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
-constexpr long long kWholeBytes = 96 << 10;
+constexpr long long kWholeBytes = 160 << 10;  // of a segment's pages
 constexpr int kAlign = 8;         // grid workgroups a segment from which segments are cut into pieces of their own
-constexpr int kItemPages = 16;    // most pages of a work item
+constexpr int kItemPages = 16;    // pages of a work item
 
 // Pages on their way: each wavefront keeps a ring of whole (page, KV head) blocks in LDS, filled by direct loads
 // (no registers, no LDS stores) several pages ahead of the pair it works on.
@@ -732,12 +732,18 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     const size_t lds = ring_bytes(d) + (size_t)(a.batch + 1) * 4 + 2048;
     const int per_cu = std::max(1, std::min<int>(regs, (int)((160 << 10) / lds)));
     p.grid = std::min(cus * per_cu, kMaxRuns - 1);
-    // Items of 16 pages, halved while the launch's most items would not give every workgroup eight.
-    const long long seg_pages = (long long)a.batch * n_seg * a.use_pages;
-    int ip = kItemPages;
-    while (ip > 1 && seg_pages / ip < 8LL * p.grid) ip >>= 1;
-    // A short segment is one item: read by one workgroup in less time than a merge's launch takes.
-    if ((long long)a.use_pages * q4_block_bytes(d) <= kWholeBytes) ip = std::max(ip, a.use_pages);
+    // Items of 16 pages, four for each wavefront: in smaller ones the wavefronts work on half pairs and the merge joins
+    // more runs (one sequence of 4000 tokens, D 256, 2 KV heads: 36 us with single pages, 16 with 16).  With 2 to 8
+    // items a workgroup the last one weighs, and 8 pages are better (16 sequences of 2000, 32 KV heads: 40 against
+    // 41.6 us); below, 8 lose to 16 (one of 32k, 8 KV heads: 25.8 against 22.9).
+    const long long items = (long long)a.batch * n_seg * a.use_pages / kItemPages;
+    int ip = items >= 2LL * p.grid && items < 8LL * p.grid ? kItemPages / 2 : kItemPages;
+    // A short segment is one item, read by one workgroup in less time than the runs of several and their merge
+    // take; one half longer counts as short where there is a segment for every CU.  (16-bit rows, 8 KV heads, D 128:
+    // 128 sequences of 992 tokens, 140 KB: 46 us cut, 38 whole; 32 of 1552, 218 KB: 26 and 19; but one sequence of
+    // that length at D 64: 16.5 and 21, and 32 of 3400, 480 KB, with the shortest a quarter of it: 28.5 and 30.)
+    const long long whole = (long long)a.batch * n_seg >= cus ? kWholeBytes * 3 / 2 : kWholeBytes;
+    if ((long long)a.use_pages * q4_block_bytes(d) <= whole) ip = std::max(ip, a.use_pages);
     a.item_pages = ip;
     p.merge = a.use_pages > ip;
     p.n_slots = (long long)a.batch * n_seg + p.grid;
