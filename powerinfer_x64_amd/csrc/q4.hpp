@@ -133,6 +133,9 @@ template <> struct Words<1> {
     __device__ __forceinline__ void load(const char* p) { w[0] = *reinterpret_cast<const uint32_t*>(p); }
 };
 
+// One of a word's two f16. By a shift: an element of the word taken as a vector sends the words through scratch memory.
+__device__ __forceinline__ f16 half_of(uint32_t w, int i) { return __builtin_bit_cast(f16, (uint16_t)(w >> (16 * i))); }
+
 // Scale words: an exact f16 on the format's grid whatever the bits were (records come from callers).
 __device__ __forceinline__ uint16_t q4_clean_scale(uint16_t bits) {
     const uint16_t mag = bits & 0x7ff0u, sign = bits & 0x8000u;

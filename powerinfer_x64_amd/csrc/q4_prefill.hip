@@ -13,10 +13,20 @@
 // odd chunks / halves are shifted by 256 bytes so that a dequantising wavefront's stores and the operand reads both
 // cover all banks.
 //
-// Schedule (8 wavefronts, two a SIMD): in step t wavefronts 0..3 run the products (PV of tile t - 1, QK of tile t) and
-// then the softmax of tile t and the unpacking of K tile t + 1; wavefronts 4..7 run the softmax of tile t - 1 and the
-// unpacking of V tile t first and the products after: on each SIMD one wavefront's matrix instructions run beside the
-// other's vector instructions.  One barrier a step.
+// Schedule of 8 wavefronts, two a SIMD (16-bit rows at D 64 and 128, f32 at 64): in step t wavefronts 0..3 run the products
+// (PV of tile t - 1, QK of tile t) and then the softmax of tile t and the unpacking of K tile t + 1; wavefronts 4..7 run
+// the softmax of tile t - 1 and the unpacking of V tile t first and the products after: on each SIMD one wavefront's
+// matrix instructions run beside the other's vector instructions.  One barrier a step.
+// Schedule of 4, one a SIMD with all its registers (D 256, f32 at 128): in step t the exps of tile t are written between
+// the matrix instructions of QK t + 1, and the unpacking of K t + 2 and V t + 1 between those of PV t, in fixed order.
+// (Against QK, softmax, PV and unpacking one after the other: 16-bit D 256 581 -> 714 TFLOP/s, f32 D 128 400 -> 470, f32
+// D 256 349 -> 414.  Two such workgroups a CU at 16-bit D 128 reach 683 where 8 wavefronts reach 838: every code is unpacked
+// for 128 rows, not 256.)
+//
+// Bound: the matrix cores' rate under load (a matrix product of 8192 cubed reaches 1230 TFLOP/s) and, at D 256, LDS reads, which
+// take as long as the products.  One sequence, 1000 rows over 8200 keys, 32 / 8 heads, back to back: D 64 115 us
+// (618 TFLOP/s: exps weigh twice), D 128 163-171 us (830-875), f32 D 128 303 us (470, each product twice);
+// 16 / 2 heads, D 256: 200 us (714), f32 344 us (414).  An 8 us merge is in them (two key splits).
 //
 // Softmax: exps against the running max as it stands; only where a row's sum of a tile passes 2^13 (the first
 // tile, or a score outgrew the max) is the tile's max taken, O and l rescaled and the tile done again.
@@ -52,11 +62,14 @@ struct KPart {
         w.load(blk + lane * (4 * NJ));
         s.load(blk + 16 * D + (lane & 15) * (2 * NJ));
     }
+    // word j to p = tile + at(page, lane)
+    static __device__ __forceinline__ int at(int page, int lane) { return k_addr<D>(lane >> 4, page * 16 + (lane & 15)); }
+    __device__ __forceinline__ void put1(int j, char* p, const Q4Magic& mg) const {
+        *reinterpret_cast<f16x8*>(p + j * (4 * kTile * 16)) = deq_k(w.w[j], half_of(s.w[j / 2], j & 1), mg);
+    }
     __device__ __forceinline__ void put(char* tile, int page, int lane, const Q4Magic& mg) const {
-        const int g = lane >> 4, key = page * 16 + (lane & 15);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-            *reinterpret_cast<f16x8*>(tile + k_addr<D>(4 * j + g, key)) = deq_k(w.w[j], __builtin_bit_cast(f16x2, s.w[j / 2])[j & 1], mg);
+        for (int j = 0; j < NJ; ++j) put1(j, tile + at(page, lane), mg);
     }
 };
 template <int D>
@@ -68,20 +81,22 @@ struct VPart {
         w.load(blk + 8 * D + lane * (4 * NJ));
         s.load(blk + 17 * D + (lane >> 4) * (8 * NJ));
     }
-    __device__ __forceinline__ void put(char* tile, int page, int lane, const Q4Magic& mg) const {
-        const int q = lane >> 4, m = lane & 15;
+    static __device__ __forceinline__ int at(int page, int lane) {
+        return v_addr<D>(page, (lane >> 4) & 1, lane & 15) + (lane >> 5) * 8;
+    }
+    __device__ __forceinline__ void put1(int j, char* p0, char* p1, const Q4Magic& mg) const {  // p1: 16 channels on
         const f16 off = (f16)-72.0f;
+        const f16x2 a = __builtin_bit_cast(f16x2, s.w[2 * j]), b = __builtin_bit_cast(f16x2, s.w[2 * j + 1]);
+        const f16x2 oa = a * off, ob = b * off;
+        const uint32_t x = w.w[j];
+        const f16x2 l0 = deq_pair(x << 4, a, oa, mg), l1 = deq_pair(x >> 4, b, ob, mg);
+        const f16x2 h0 = deq_pair(x, a, oa, mg), h1 = deq_pair(x >> 8, b, ob, mg);
+        *reinterpret_cast<f16x4*>(p0 + j * 512) = f16x4{l0[0], l0[1], l1[0], l1[1]};
+        *reinterpret_cast<f16x4*>(p1 + j * 512) = f16x4{h0[0], h0[1], h1[0], h1[1]};
+    }
+    __device__ __forceinline__ void put(char* tile, int page, int lane, const Q4Magic& mg) const {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const f16x2 a = __builtin_bit_cast(f16x2, s.w[2 * j]), b = __builtin_bit_cast(f16x2, s.w[2 * j + 1]);
-            const f16x2 oa = a * off, ob = b * off;
-            const uint32_t x = w.w[j];
-            const f16x2 l0 = deq_pair(x << 4, a, oa, mg), l1 = deq_pair(x >> 4, b, ob, mg);
-            const f16x2 h0 = deq_pair(x, a, oa, mg), h1 = deq_pair(x >> 8, b, ob, mg);
-            char* p = tile + (q >> 1) * 8;
-            *reinterpret_cast<f16x4*>(p + v_addr<D>(page, q & 1, 32 * j + m)) = f16x4{l0[0], l0[1], l1[0], l1[1]};
-            *reinterpret_cast<f16x4*>(p + v_addr<D>(page, q & 1, 32 * j + 16 + m)) = f16x4{h0[0], h0[1], h1[0], h1[1]};
-        }
+        for (int j = 0; j < NJ; ++j) put1(j, tile + at(page, lane), tile + (at(page, lane) ^ 256), mg);
     }
 };
 
@@ -193,7 +208,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
     // Both products read their LDS operands kAhead ahead, one read beside each matrix instruction (left alone, the
     // compiler requests them all first and spills).
     constexpr int kAhead = 4;
-    auto paced = [](int n) {
+    auto plain = [](int n) {
         __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
         for (int i = 0; i < 64; ++i)
@@ -203,7 +218,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
             }
         __builtin_amdgcn_sched_group_barrier(0x008, kAhead * PREC, 0);
     };
-    auto qk = [&](int t) {
+    auto none = [](auto&&...) {};
+    auto qk = [&](int t, f32x16 (&s)[2], auto&& also, auto&& pace) {
         const char* tile = lds + (t & 1) * kBuf + k_addr<D>(hh, col);
         auto frag = [&](int i) {  // chunk 2 (i / 2) + hh, keys 32 (i % 2) + col
             return *reinterpret_cast<const f16x8*>(tile + (i >> 1) * (2 * kTile * 16) + (i & 1) * 512);
@@ -219,10 +235,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
             if (i + kAhead < 2 * KS) f[i % kAhead] = frag(i + kAhead);
 #pragma unroll
             for (int h = 0; h < PREC; ++h) s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[h][i >> 1], s[i & 1], 0, 0, 0);
+            also(i);
         }
-        paced(2 * KS);
+        pace(2 * KS);
     };
-    auto pv = [&](int t) {
+    auto pv = [&](int t, auto&& also, auto&& pace) {
         // page i / NB, half hh, channel (32 (i % NB) + col) ^ 16 hh
         const char* tile = lds + (2 + (t & 1)) * kBuf + v_addr<D>(0, hh, col);
         auto frag = [&](int i) { return *reinterpret_cast<const f16x8*>(tile + (i / NB) * (2 * D * 16) + (i % NB) * 512); };
@@ -236,8 +253,9 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
 #pragma unroll
             for (int h = 0; h < PREC; ++h)
                 o[i % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[h][i / NB], o[i % NB], 0, 0, 0);
+            also(i);
         }
-        paced(4 * NB);
+        pace(4 * NB);
     };
     // P of the tile against m, its sum over the lane's 32 keys.
     auto exps = [&] {
@@ -258,7 +276,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
         }
         return (part[0] + part[1]) + (part[2] + part[3]);
     };
-    auto softmax = [&](int t, uint32_t bad) {
+    auto mask = [&](int t, uint32_t bad) {
         if (bad != 0 || (t + 1) * kTile > lim_all) {  // scores that do not count: -inf after the factor, which is not 0
             const int left = lim - t * kTile - 4 * hh;
             const float none = back < 0.f ? INFINITY : -INFINITY;
@@ -268,7 +286,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
                 for (int e = 0; e < 16; ++e)
                     if (32 * kb + 8 * (e >> 2) + (e & 3) >= left || ((bad >> (2 * kb + (e >> 3))) & 1)) s[kb][e] = none;
         }
-        float sum = exps();
+    };
+    auto add = [&](float sum) {
         if (__any(sum > kRedo)) {  // no P is above 1 after it
             float mx = -1e30f;
 #pragma unroll
@@ -284,6 +303,10 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
             sum = exps();
         }
         l += sum;
+    };
+    auto softmax = [&](int t, uint32_t bad) {
+        mask(t, bad);
+        add(exps());
     };
 
     auto finish = [&] {
@@ -361,20 +384,20 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
             };
             step_ids(t0);
             if (n > t0) {
-                qk(t0);
+                qk(t0, s, none, plain);
                 softmax(t0, bad);
             }
             unpack(t0);
             for (int t = t0 + 1; t < n; ++t) {
                 step_ids(t);
                 __builtin_amdgcn_s_setprio(2);
-                pv(t - 1);
-                qk(t);
+                pv(t - 1, none, plain);
+                qk(t, s, none, plain);
                 __builtin_amdgcn_s_setprio(0);
                 softmax(t, bad);
                 unpack(t);
             }
-            if (n > t0) pv(n - 1);
+            if (n > t0) pv(n - 1, none, plain);
             for (int t = max(n, t0 + 1); t <= t1; ++t) {
                 step_ids(t);
                 unpack(t);
@@ -392,7 +415,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
             };
             step_ids(t0);
             unpack(t0);
-            if (n > t0) qk(t0);
+            if (n > t0) qk(t0, s, none, plain);
             barrier_lds();
             uint32_t was = bad;
             for (int t = t0 + 1; t < n; ++t) {
@@ -401,8 +424,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
                 softmax(t - 1, was);
                 was = bad;
                 __builtin_amdgcn_s_setprio(2);
-                pv(t - 1);
-                qk(t);
+                pv(t - 1, none, plain);
+                qk(t, s, none, plain);
                 __builtin_amdgcn_s_setprio(0);
                 barrier_lds();
             }
@@ -411,7 +434,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
                 step_ids(n);
                 unpack(n);
                 softmax(n - 1, was);
-                pv(n - 1);
+                pv(n - 1, none, plain);
                 barrier_lds();
                 t = n + 1;
             }
@@ -425,21 +448,87 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void q4_tile_kernel(Q4AttnArgs a, 
     } else {
         KPart<D> kp;
         VPart<D> vp;
+        int i3 = ids_of(t0 + 2), i4 = ids_of(t0 + 3);  // of tiles t + 2, t + 3 (i1, i2: t, t + 1)
+        auto put_k = [&](int t) { kp.put(lds + (t & 1) * kBuf, wave, lane, mg); };
+        auto put_v = [&](int t) { vp.put(lds + (2 + (t & 1)) * kBuf, wave, lane, mg); };
+        auto next = [&](int t) {  // pages of step t + 1
+            kp.load(block_of(i4, wave), lane);
+            vp.load(block_of(i3, wave), lane);
+            i1 = i2;
+            i2 = i3;
+            i3 = i4;
+            i4 = ids_of(t + 4);
+        };
+        // beside the second product: every second step a word of the next K or V codes
+        auto put_some = [&](int t) {
+            // opaque: left alone, the compiler keeps an address for every word, in scratch memory
+            int ko = (t & 1) * kBuf + KPart<D>::at(wave, lane), vo = (2 + ((t + 1) & 1)) * kBuf + VPart<D>::at(wave, lane), vx = vo ^ 256;
+            asm volatile("" : "+v"(ko), "+v"(vo), "+v"(vx));
+            return [&, ko, vo, vx](int i) {
+                constexpr int NJ = D / kQ4Group;
+                const int j = i / 2;
+                if (i & 1) {
+                } else if (j < NJ) kp.put1(j, lds + ko, mg);
+                else vp.put1(j - NJ, lds + vo, lds + vx, mg);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+        };
         kp.load(block_of(i1, wave), lane);
         vp.load(block_of(i1, wave), lane);
-        for (int t = t0; t < t1; ++t) {
-            step_ids(t);
-            // the other halves of the buffers may still be read in step t - 1, these by no wavefront
-            kp.put(lds + (t & 1) * kBuf, wave, lane, mg);
-            vp.put(lds + (2 + (t & 1)) * kBuf, wave, lane, mg);
+        put_k(t0);
+        put_v(t0);
+        kp.load(block_of(i2, wave), lane);
+        vp.load(block_of(i2, wave), lane);
+        put_k(t0 + 1);
+        kp.load(block_of(i3, wave), lane);
+        barrier_lds();
+        if (n > t0) qk(t0, s, none, plain);
+        barrier_lds();
+        int t = t0;
+        for (; t < n - 1; ++t) {
+            mask(t, bad_of(i1));
+            f32x16 sn[2];
+            float sum = 0.f, even = 0.f;
+            qk(t + 1, sn, [&](int i) {
+                constexpr int E = 16 / KS;  // scores a step
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    const int k = E * i + j, st = k >> 3, e = k & 7;
+                    const float x = fast_exp2(fmaf(s[st >> 1][8 * (st & 1) + ((e & 4) | ((e & 1) << 1) | ((e >> 1) & 1))], back, -m));
+                    sum += x;
+                    if (!(e & 1)) {
+                        even = x;
+                        continue;
+                    }
+                    const f16 h0 = to_f16(even), h1 = to_f16(x);
+                    pf[0][st][e - 1] = h0;
+                    pf[0][st][e] = h1;
+                    if (PREC == 2) {
+                        pf[PREC - 1][st][e - 1] = to_f16(even - (float)h0);
+                        pf[PREC - 1][st][e] = to_f16(x - (float)h1);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }, none);
+            add(sum);
+            pv(t, put_some(t), none);
+            next(t);
+            s[0] = sn[0];
+            s[1] = sn[1];
             barrier_lds();
-            kp.load(block_of(i1, wave), lane);
-            vp.load(block_of(i1, wave), lane);
-            if (t < n) {
-                qk(t);
-                softmax(t, bad);
-                pv(t);
-            }
+        }
+        if (n > t0) {
+            softmax(t, bad_of(i1));
+            pv(t, put_some(t), none);
+            next(t);
+            ++t;
+            barrier_lds();
+        }
+        for (; t < t1; ++t) {
+            put_k(t + 2);
+            put_v(t + 1);
+            next(t);
+            barrier_lds();
         }
         finish();
     }
