@@ -452,7 +452,8 @@ void pi_rope_plan_destroy(pi_rope_plan plan);
 /* Rotates q, and k unless d_k is NULL, at positions d_pos[n_tok].  Element (token t, head h, channel d) of
  * a tensor lies at t * tok + h * head + d, strides in elements (any order and alignment; rows of 16-byte
  * aligned chunks take the vector kernel).  An output is either its input with the same
- * strides (in place) or shares no memory with it. */
+ * strides (in place) or shares no memory with it, and none with the other tensors.  n_tok below 2^24,
+ * (n_q_heads + n_kv_heads) * head_dim up to 2^30. */
 int pi_rope_apply(pi_handle h, pi_rope_plan plan, int32_t dtype, int32_t n_tok, int32_t head_dim,
                   const int32_t* d_pos, const void* d_q, int64_t q_tok, int64_t q_head,
                   int32_t n_q_heads, void* d_q_out, int64_t qo_tok, int64_t qo_head, const void* d_k,
@@ -483,8 +484,8 @@ size_t pi_q4_pool_bytes(pi_q4_pool pool);
  * token (n_rows = n_seq).  Rows of no sequence are neither read nor written anywhere.  Inputs as in
  * pi_rope_apply (strides in elements); d_q may be NULL (k and v alone); d_q_out shares no memory with the
  * inputs.  d_k_values, d_v_values (each NULL or f16 [n_rows][n_kv_heads][head_dim], 16-byte aligned) receive the
- * values that the cache now holds, for pi_attn_prefill over a fresh prompt.  n_seq <= 4096.  One call must not
- * store two tokens in one slot (a page in two rows of the table is fine for reading). */
+ * values that the cache now holds, for pi_attn_prefill over a fresh prompt.  n_seq <= 4096, n_rows below 2^24.
+ * One call must not store two tokens in one slot (a page in two rows of the table is fine for reading). */
 int pi_q4_append(pi_handle h, pi_q4_pool pool, pi_rope_plan plan, int32_t dtype, int32_t n_rows,
                  const int32_t* d_tok_start, const int32_t* d_start_pos, int32_t n_seq,
                  const int32_t* d_page_table, int32_t max_pages, const void* d_q, int64_t q_tok,
@@ -507,7 +508,8 @@ int pi_q4_write(pi_handle h, pi_q4_pool pool, const int32_t* d_page_table, int32
 /* Attention over the cache (src/model/mod.rs:1148-1196): softmax(scale q.k) v over each row's keys, times
  * sigmoid(gate) where d_gate is not NULL; f32 softmax and sums, q, gate and out all in dtype (f32, f16 or bf16;
  * f32 rows keep f32 accuracy).  Head maps as pi_attn_decode.  A row without keys gets zeros.
- * q, gate, out and the workspace are 16-byte aligned and contiguous.
+ * q, gate, out and the workspace are 16-byte aligned and contiguous, and out and the workspace share no
+ * memory with the others.
  * max_ctx: no sequence holds more tokens (0: 16 * max_pages); a longer one is cut to it, rounded up to whole
  * pages.  A small max_ctx on a wide table saves a launch.
  * The workspace is the caller's, of at least pi_q4_attn_ws_bytes for the same arguments (0: NULL will do; for
@@ -525,8 +527,8 @@ int pi_q4_attn_decode(pi_handle h, pi_q4_pool pool, const void* d_q, int32_t dty
                       float scale, const void* d_gate, void* d_out, void* d_ws, size_t ws_bytes,
                       void* stream);
 /* A chunk of tokens a sequence, causal: rows as in pi_q4_append, row i of sequence s sees keys 0 ..
- * d_start_pos[s] + i (its chunk appended first).  No sequence has more than max_tok rows; the rows of a
- * longer one past max_tok, and rows of no sequence, are left as they were.  n_seq <= 4096. */
+ * d_start_pos[s] + i (its chunk appended first).  No sequence has more than max_tok rows (a close bound
+ * launches fewer workgroups); the rows of a longer one past max_tok, and rows of no sequence, are left as they were.  n_seq <= 4096. */
 int pi_q4_attn_prefill(pi_handle h, pi_q4_pool pool, const void* d_q, int32_t dtype, int32_t n_rows,
                        const int32_t* d_tok_start, const int32_t* d_start_pos, int32_t n_seq,
                        int32_t max_tok, const int32_t* d_page_table, int32_t max_pages,

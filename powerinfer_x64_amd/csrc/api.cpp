@@ -1991,6 +1991,9 @@ int pi_rope_apply(pi_handle h, pi_rope_plan plan, int32_t dtype, int32_t n_tok, 
     if (dtype < PI_F32 || dtype > PI_BF16) return fail(h, PI_ERR_UNSUPPORTED, "pi_rope_apply: dtype %d", dtype);
     if (n_tok < 0 || n_q_heads <= 0 || n_kv_heads < (d_k ? 1 : 0) || n_q_heads > 65536 || n_kv_heads > 65536)
         return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: n_tok=%d heads=%d/%d", n_tok, n_q_heads, n_kv_heads);
+    // a launch's threads a dimension, and a token's units in the kernels, are 32 bits
+    if (n_tok >= 1 << 24 || ((int64_t)n_q_heads + n_kv_heads) * head_dim > 1 << 30)
+        return fail(h, PI_ERR_UNSUPPORTED, "pi_rope_apply: %d tokens of %d + %d heads of %d", n_tok, n_q_heads, n_kv_heads, head_dim);
     if (head_dim < 2 * plan->p.half || head_dim > 65536)
         return fail(h, PI_ERR_INVALID_ARG, "pi_rope_apply: head_dim %d for a plan of %d channels", head_dim, 2 * plan->p.half);
     if (q_tok < 0 || q_head < 0 || (d_k && (k_tok < 0 || k_head < 0)))
@@ -2024,7 +2027,7 @@ int pi_q4_pool_create(pi_handle h, int32_t n_pages, int32_t page_tokens, int32_t
     *out = nullptr;
     if (page_tokens != pi::kPageTokens)
         return fail(h, PI_ERR_UNSUPPORTED, "pi_q4_pool_create: page_tokens must be 16 (got %d)", page_tokens);
-    if (n_pages <= 0 || n_kv_heads <= 0)
+    if (n_pages <= 0 || n_kv_heads <= 0 || n_kv_heads > 65536)
         return fail(h, PI_ERR_INVALID_ARG, "pi_q4_pool_create: n_pages=%d n_kv_heads=%d", n_pages, n_kv_heads);
     if (!dim_ok(head_dim)) return fail(h, PI_ERR_UNSUPPORTED, "pi_q4_pool_create: head_dim %d (64/128/256)", head_dim);
     const DeviceScope on(h->device);
@@ -2074,6 +2077,7 @@ int pi_q4_append(pi_handle h, pi_q4_pool pool, pi_rope_plan plan, int32_t dtype,
         n_q_heads > 65536)
         return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: n_rows=%d n_seq=%d (at most %d) max_pages=%d n_q_heads=%d", n_rows, n_seq,
                     pi::kQ4MaxBatch, max_pages, n_q_heads);
+    if (n_rows >= 1 << 24) return fail(h, PI_ERR_UNSUPPORTED, "pi_q4_append: %d rows (below 2^24)", n_rows);
     if (!d_tok_start && n_rows != n_seq)
         return fail(h, PI_ERR_INVALID_ARG, "pi_q4_append: %d rows for %d sequences of one token each", n_rows, n_seq);
     if (plan && 2 * plan->p.half > g.head_dim)
@@ -2194,6 +2198,8 @@ int q4_attn(pi_handle h, const char* what, pi_q4_pool pool, const void* d_q, int
     if (!d_q || !d_out || !d_pos || !d_page_table) return fail(h, PI_ERR_INVALID_ARG, "%s: null argument", what);
     for (const void* p : {d_q, d_gate, static_cast<const void*>(d_out), static_cast<const void*>(d_ws)})
         if (reinterpret_cast<uintptr_t>(p) % 16) return fail(h, PI_ERR_INVALID_ARG, "%s: q, gate, out and ws must be 16-byte aligned", what);
+    if (d_out == d_q || d_out == d_gate || d_out == d_ws)
+        return fail(h, PI_ERR_INVALID_ARG, "%s: out must be another tensor than q, gate and ws", what);
     if (plan.ws_bytes && (!d_ws || ws_bytes < plan.ws_bytes))
         return fail(h, PI_ERR_INVALID_ARG, "%s: the workspace holds %zu bytes, %zu are needed", what, d_ws ? ws_bytes : (size_t)0,
                     plan.ws_bytes);

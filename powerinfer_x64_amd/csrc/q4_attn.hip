@@ -666,10 +666,10 @@ hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStrea
     }
     const int stage = stage_floats(a.cols, D);
     const size_t lds = ring_bytes(D) + (size_t)(a.batch + 1) * 4;
-    if (lds > (64 << 10)) {  // more than a kernel may ask for without saying so
-        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_attn_kernel<T, D, NCB>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                        (int)(ring_bytes(D) + (kQ4MaxBatch + 1) * 4));
+    if (lds > (64 << 10)) {
+        static std::atomic<uint64_t> on{0};
+        const hipError_t e =
+            allow_lds(reinterpret_cast<const void*>(&q4_attn_kernel<T, D, NCB>), ring_bytes(D) + (kQ4MaxBatch + 1) * 4, on);
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL((q4_attn_kernel<T, D, NCB>), dim3(plan.grid), dim3(kThreads), lds, s, a, ws, stage);
@@ -715,9 +715,11 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
         // Few row blocks: their keys are split while that fills idle CUs and each part keeps 4 tiles.
         long long splits = wgs >= cus ? 1 : std::min<long long>({kMaxSplits, cus / wgs, a.use_pages / 16});
         splits = std::max<long long>(splits, 1);
+        // (a merge of mostly rows of no sequence may be more threads than a launch takes)
+        if ((long long)a.n_rows * a.n_q_heads * (d / 4) >= 1ll << 32) splits = 1;
         p.splits = (int)splits;
         p.n_blk = (int)n_blk;
-        p.grid = wgs * splits > 0x7fffffffll ? 0 : (int)(wgs * splits);  // 0: the caller refuses
+        p.grid = wgs * splits * 512 >= 1ll << 32 ? 0 : (int)(wgs * splits);  // a launch's most threads; 0: the caller refuses
         p.merge = splits > 1;
         p.ws_bytes = p.merge ? (size_t)splits * a.n_rows * a.n_q_heads * (d + 2) * 4 : 0;
         return p;

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "q4.hpp"
 
 namespace pi {
@@ -81,6 +83,16 @@ struct Q4Plan {
     long long n_slots;
     size_t ws_bytes;
 };
+// Lets a kernel ask for more than 64 KB of LDS, on every device it runs on: `on` has a bit for each where it may.
+inline hipError_t allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& on) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e != hipSuccess || (on.load(std::memory_order_relaxed) & bit)) return e;
+    e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == hipSuccess) on.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 // Fills a's planned fields.
 Q4Plan q4_plan(Q4AttnArgs& a, int device);
 hipError_t launch_q4_attn(const Q4AttnArgs& a, const Q4Plan& plan, void* ws, hipStream_t s);

@@ -597,8 +597,8 @@ template <typename T, int D, int NW>
 hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& p, const TileArgs& ta, hipStream_t s) {
     const size_t lds = (size_t)4 * kTile * D * 2;
     if (lds > (64 << 10)) {
-        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&q4_tile_kernel<T, D, NW>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        static std::atomic<uint64_t> on{0};
+        const hipError_t e = allow_lds(reinterpret_cast<const void*>(&q4_tile_kernel<T, D, NW>), lds, on);
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL((q4_tile_kernel<T, D, NW>), dim3((unsigned)p.grid), dim3(NW * 64), lds, s, a, ta);

@@ -786,6 +786,8 @@ def rope_apply(dev: Device, plan: RopePlan, q: torch.Tensor, k: Optional[torch.T
     themselves for a rotation in place.  Returns (q_out, k_out)."""
     code, td, dt, shape = _float_rows(q, "q"), dev.torch_device, q.dtype, q.shape
     n, hq, d = shape
+    if not plan.p:
+        raise InvalidArg("plan: closed")
     qp = _rows(q, "q", dt, shape, td)
     if q_out is None:
         q_out = torch.empty_like(q)
@@ -849,6 +851,8 @@ class Q4Pool:
         with `values`, (q_out, k, v) with the f16 [n, Hkv, D] values that the cache now holds (rows of no
         sequence stay uninitialised)."""
         d, td = self.dev, self.dev.torch_device
+        if plan is not None and not plan.p:
+            raise InvalidArg("plan: closed")  # (a null plan is no rotation)
         code = _float_rows(k, "k")
         dt, n, dh = k.dtype, k.shape[0], self.head_dim
         shape = (n, self.n_kv_heads, dh)
@@ -970,7 +974,7 @@ def q4_attn_prefill(dev: Device, q: torch.Tensor, pool: Q4Pool, page_table: torc
                     ws: Optional[torch.Tensor] = None):
     """A chunk of tokens a sequence, causal: q [n, Hq, D], sequence s's rows tok_start[s] .. tok_start[s + 1] - 1
     at positions start_pos[s] ... (their keys appended first) -> out like q.  max_tok: no sequence has more
-    rows (default: n).  Rows of no sequence are left as they were in `out`."""
+    rows (default: n; a close bound launches fewer workgroups).  Rows of no sequence are left as they were in `out`."""
     n_seq = start_pos.shape[0] if isinstance(start_pos, torch.Tensor) and start_pos.dim() == 1 else -1
     n = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() else 0
     if start_pos is None or tok_start is None:

@@ -696,3 +696,62 @@ def test_refusals():
     assert empty.shape == (0, 4, 128)
     assert rt.q4_attn_prefill(dev, q[:0], pool, pt, pos, i32([0, 0, 0])).shape == (0, 4, 128)
     assert all(t.shape[0] == 0 for t in pool.read(pt, 0, 0, 0))
+
+
+# ---- choices of the launch, and what it refuses ------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv,n,top", [("f16", 128, 8, 2, 140, 1500), ("f32", 64, 4, 4, 70, 2000), ("bf16", 256, 16, 16, 24, 1500),
+                                                  ("f16", 64, 32, 32, 24, 4000)])
+def test_decode_many_segments(dtype, d, hq, hkv, n, top):
+    """A segment for every CU: whole ones up to a size, items of half the pages past it."""
+    lens = np.random.default_rng(n).integers(0, top + 1, n).tolist()
+    lens[3], lens[-1] = top, 0
+    check_decode(dtype, d, hq, hkv, lens, seed=n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_prefill_many_splits(dtype, d):
+    """Few row blocks over long histories: up to 32 key splits, some of them empty, joined by the merge."""
+    check_prefill(dtype, d, 8, 2, [40], [9000], seed=d)
+    check_prefill(dtype, d, 8, 2, [3, 0, 70], [9000, 5, 1], gate=True, seed=d + 1)
+
+
+def test_prefill_many_sequences_merge():
+    """More sequences than the lanes of a row: the merge finds each row's."""
+    rng = np.random.default_rng(31)
+    toks = rng.integers(0, 20, 100)
+    toks[50] = 20
+    check_prefill("f16", 64, 4, 1, toks.tolist(), rng.integers(0, 1200, 100).tolist(), seed=31, max_tok=20)
+
+
+def test_closed_plans_shared_outputs_and_sizes_are_refused():
+    dev = device()
+    pool = rt.Q4Pool(dev, 8, 2, 128)
+    pt = i32([[0, 1], [2, 3]])
+    kv = torch.zeros(2, 2, 128, device="cuda", dtype=torch.float16)
+    q = torch.zeros(2, 4, 128, device="cuda", dtype=torch.float16)
+    gate = torch.zeros_like(q)
+    plan = rt.RopePlan(dev, 128)
+    plan.close()
+    with pytest.raises(rt.InvalidArg, match="closed"):
+        pool.append(kv, kv, pt, i32([0, 0]), plan=plan)
+    with pytest.raises(rt.InvalidArg, match="closed"):
+        rt.rope_apply(dev, plan, q, None, i32([0, 0]))
+    for kw in (dict(out=q), dict(gate=gate, out=gate)):
+        with pytest.raises(rt.InvalidArg, match="another tensor"):
+            rt.q4_attn_decode(dev, q, pool, pt, i32([1, 1]), **kw)
+        with pytest.raises(rt.InvalidArg, match="another tensor"):
+            rt.q4_attn_prefill(dev, q, pool, pt, i32([0, 0]), i32([0, 1, 2]), **kw)
+    with pytest.raises(rt.InvalidArg):
+        rt.Q4Pool(dev, 1, 1 << 17, 64)
+    plan, p, unsupported = rt.RopePlan(dev, 64), q.data_ptr(), 5  # PI_ERR_UNSUPPORTED
+    size = lambda n, d, h: dev.lib.pi_rope_apply(dev.h, plan.p, rt.F16, n, d, p, p, h * d, d, h, p, h * d, d, None, 0, 0, 0, None, 0, 0,  # noqa: E731
+                                                 dev.stream())
+    assert [size(1 << 24, 64, 1), size(1, 65536, 16385)] == [unsupported] * 2
+    rows = (1 << 24, i32([0, 1]).data_ptr(), i32([0]).data_ptr(), 1, pt.data_ptr(), 2)
+    assert dev.lib.pi_q4_append(dev.h, pool.p, None, rt.F16, *rows, None, 0, 0, 0, None, 0, 0, p, 256, 128, p, 256, 128, None, None, 0.0,
+                                None, None, dev.stream()) == unsupported
+    need = ctypes.c_size_t()
+    assert dev.lib.pi_q4_attn_ws_bytes(dev.h, pool.p, rt.F16, 1 << 30, 4096, 1 << 30, 4, 0, 8, 0, ctypes.byref(need)) == unsupported
