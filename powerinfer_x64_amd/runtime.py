@@ -750,6 +750,13 @@ def _rows(t: torch.Tensor, name: str, dtype, shape, dev):
     raise InvalidArg(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
+def _new_rows(t: torch.Tensor):
+    """A new contiguous tensor like t, and what _rows would give for it."""
+    t = torch.empty_like(t, memory_format=torch.contiguous_format)
+    st, sh, _ = t.stride()
+    return t, (t.data_ptr(), st, sh)
+
+
 def _table(t: torch.Tensor, name: str, dtype, shape, dev):
     """A contiguous tensor's address (None: None)."""
     if t is None:
@@ -782,7 +789,7 @@ def _float_rows(t, name):
 def rope_apply(dev: Device, plan: RopePlan, q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor,
                q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
     """q [n, Hq, D] and k [n, Hkv, D] (f32 / f16 / bf16, D contiguous, any other strides) rotated at
-    positions pos int32 [n], into q_out and k_out: new tensors (torch.empty_like's) by default, or q and k
+    positions pos int32 [n], into q_out and k_out: new tensors (contiguous) by default, or q and k
     themselves for a rotation in place.  Returns (q_out, k_out)."""
     code, td, dt, shape = _float_rows(q, "q"), dev.torch_device, q.dtype, q.shape
     n, hq, d = shape
@@ -790,8 +797,9 @@ def rope_apply(dev: Device, plan: RopePlan, q: torch.Tensor, k: Optional[torch.T
         raise InvalidArg("plan: closed")
     qp = _rows(q, "q", dt, shape, td)
     if q_out is None:
-        q_out = torch.empty_like(q)
-    qo = _rows(q_out, "q_out", dt, shape, td)
+        q_out, qo = _new_rows(q)
+    else:
+        qo = _rows(q_out, "q_out", dt, shape, td)
     kp = ko = (None, 0, 0)
     hkv = 0
     if k is not None:
@@ -800,8 +808,9 @@ def rope_apply(dev: Device, plan: RopePlan, q: torch.Tensor, k: Optional[torch.T
         shape = (n, hkv, d)
         kp = _rows(k, "k", dt, shape, td)
         if k_out is None:
-            k_out = torch.empty_like(k)
-        ko = _rows(k_out, "k_out", dt, shape, td)
+            k_out, ko = _new_rows(k)
+        else:
+            ko = _rows(k_out, "k_out", dt, shape, td)
     rc = dev.lib.pi_rope_apply(dev.h, plan.p, code, n, d, _table(pos, "pos", torch.int32, (n,), td), *qp, hq, *qo, *kp, hkv,
                                *ko, dev.stream())
     if rc:
@@ -869,8 +878,9 @@ class Q4Pool:
             hq = q.shape[1]
             qp = _rows(q, "q", dt, (n, hq, dh), td)
             if q_out is None:
-                q_out = torch.empty((n, hq, dh), dtype=dt, device=td)
-            qo = _rows(q_out, "q_out", dt, (n, hq, dh), td)
+                q_out, qo = _new_rows(q)
+            else:
+                qo = _rows(q_out, "q_out", dt, (n, hq, dh), td)
         qw = _table(q_norm_w, "q_norm_w", torch.float32, (dh,), td)
         kw = _table(k_norm_w, "k_norm_w", torch.float32, (dh,), td)
         k_val = torch.empty(shape, dtype=torch.float16, device=td) if values else None
