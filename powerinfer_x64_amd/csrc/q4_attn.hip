@@ -36,6 +36,7 @@ constexpr int kStage = 1024;      // most floats a wavefront stages at a time fo
 constexpr int kMaxSplits = 32;    // key splits of a tiled row block
 constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
 constexpr long long kWholeBytes = 160 << 10;  // of a segment's pages
+static_assert(kWholeBytes * 3 / 2 / (18 * 64) <= sched::kSubPages, "a whole segment's page ids fit one load of the lanes");
 constexpr int kAlign = 8;         // grid workgroups a segment from which segments are cut into pieces of their own
 constexpr int kItemPages = 16;    // pages of a work item
 
@@ -308,7 +309,9 @@ struct LenOf {
 template <typename T, int D, int NCB>
 constexpr int min_waves() { return NCB * D * (sizeof(T) == 4 ? 3 : 2) <= 512 ? 2 : 1; }
 
-template <typename T, int D, int NCB>
+// WHOLE: no merge follows.  Workgroup i takes segments i, i + grid, .. whole, and the schedule's scan of the batch (three trips to
+// memory and back before a first page is asked for) is not needed.
+template <typename T, int D, int NCB, bool WHOLE>
 __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_kernel(Q4AttnArgs a, Q4Ws ws, int stage) {
     typedef Ring<D> R;
     // the wavefronts' rings, then s_cum[batch + 1]; the rings' space also stages O: [4][stage] floats
@@ -321,27 +324,22 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
 
     const Q4Magic mg;
     const int n_kv = a.g.n_kv_heads, n_seg = n_kv * a.n_cb, tid = threadIdx.x;
-    if (!ws.runs)  // no merge follows: the rows of sequences without keys are zeroed here
-        for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-            const Q4Rows rw = rows_of(a, b);
-            if (rw.len != 0) continue;
-            T* out = static_cast<T*>(a.out) + (size_t)rw.first * a.n_q_heads * D;
-            for (size_t i = tid; i < (size_t)rw.n * a.n_q_heads * D; i += kThreads) out[i] = from_f32<T>(0.f);
-        }
-    int n_items = n_seg * scan_items(a, s_cum, s_red, 1);
-    int chunk = (n_items + gridDim.x - 1) / gridDim.x;
-    // Few segments for the grid: each is cut into pieces of its own instead, a piece a workgroup, so that none pays the
-    // start and the end of two runs.  Pieces of `piece` items number at most the grid.
     const int segs = a.batch * n_seg;
-    int piece = 0;
-    if (ws.runs && segs * kAlign <= (int)gridDim.x) {
-        piece = max(1, (n_items + (int)gridDim.x - segs - 1) / ((int)gridDim.x - segs));
-        __syncthreads();
-        n_items = n_seg * scan_items(a, s_cum, s_red, piece);
-        chunk = 1;  // s_cum counts pieces now
+    int chunk = 1, piece = 0, cur = blockIdx.x, end = segs;
+    if constexpr (!WHOLE) {
+        int n_items = n_seg * scan_items(a, s_cum, s_red, 1);
+        chunk = (n_items + gridDim.x - 1) / gridDim.x;
+        // Few segments for the grid: each is cut into pieces of its own instead, a piece a workgroup, so that none pays the
+        // start and the end of two runs.  Pieces of `piece` items number at most the grid.
+        if (segs * kAlign <= (int)gridDim.x) {
+            piece = max(1, (n_items + (int)gridDim.x - segs - 1) / ((int)gridDim.x - segs));
+            __syncthreads();
+            n_items = n_seg * scan_items(a, s_cum, s_red, piece);
+            chunk = 1;  // s_cum counts pieces now
+        }
+        cur = blockIdx.x * chunk;
+        end = min(n_items, cur + chunk);
     }
-    int cur = blockIdx.x * chunk;
-    const int end = min(n_items, cur + chunk);
     if (cur >= end) return;
 
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -351,10 +349,25 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
     const uint32_t lane16 = lane * 16, lane4 = lane * 4;
     const uint32_t ring_at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)ring);
 
-    int b = sched::find_seq(s_cum, a.batch, n_seg, cur);
+    int b = WHOLE ? 0 : sched::find_seq(s_cum, a.batch, n_seg, cur);
     while (cur < end) {
-        sched::Run run = sched::run_of(s_cum, LenOf{a}, n_seg, a.item_pages, b, cur, end);
-        b = run.b;
+        sched::Run run;
+        int pid_first = 0;  // WHOLE: the wavefront's page ids, asked for together with the length
+        if constexpr (WHOLE) {
+            b = cur / n_seg;
+            pid_first = a.page_table[(size_t)b * a.max_pages + min(wave + kWaves * lane, a.use_pages - 1)];
+            run.b = b;
+            run.kvh = cur - b * n_seg;
+            run.seg0 = cur;
+            run.run_end = cur + gridDim.x;
+            run.len = rows_of(a, b).len;
+            run.pg0 = 0;
+            run.pg1 = (run.len + sched::kPage - 1) / sched::kPage;
+            run.whole = true;
+        } else {
+            run = sched::run_of(s_cum, LenOf{a}, n_seg, a.item_pages, b, cur, end);
+            b = run.b;
+        }
         if (piece) {  // the segment's pages in equal pieces
             const int k = s_cum[b + 1] - s_cum[b], pages = (run.len + sched::kPage - 1) / sched::kPage;
             const int i = cur - run.seg0, each = (pages + k - 1) / k;
@@ -364,7 +377,7 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
         const int sidx = run.kvh, kvh = sidx / a.n_cb, row0 = (sidx % a.n_cb) * a.cols;
         const Q4Rows rw = rows_of(a, b);
         const size_t seg = (size_t)b * n_seg + sidx;
-        if (cur == run.seg0 && tid == 0 && ws.runs) {
+        if (cur == run.seg0 && !WHOLE && tid == 0) {
             int wg1;
             const int n_runs = sched::merge_runs(s_cum, n_seg, chunk, b, sidx, &wg1);
             ws.runs[2 * seg] = wg1;
@@ -396,7 +409,7 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
                 int first, n_my;
                 sched::sub_pages(sub, run.pg1, wave, &first, &n_my);
                 // A page id outside the pool holds no tokens: page 0 is read in its place, all of it masked.
-                const int pid_raw = lane < n_my ? pt[first + kWaves * lane] : 0;
+                const int pid_raw = lane >= n_my ? 0 : WHOLE ? pid_first : pt[first + kWaves * lane];
                 const bool bad = !sched::page_ok(pid_raw, a.g.n_pages);
                 const int pid_v = bad ? 0 : pid_raw;
                 const uint64_t bad_pages = __ballot(bad);
@@ -521,7 +534,7 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
                     if (off < 0) continue;
                     typedef T t4 __attribute__((ext_vector_type(4)));
                     t4 y;
-                    if (a.gate) {
+                    if (a.gate && run.len) {  // (rows without keys get zeros)
                         const t4 g = *reinterpret_cast<const t4*>(static_cast<const T*>(a.gate) + off + d);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[e] *= sigmoidf_(to_f32(g[e]));
@@ -629,7 +642,7 @@ template <typename T, int D, int NCB>
 int vgpr_wgs() {  // resident workgroups a CU by registers alone
     static const int n = [] {
         int v = 0;
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, q4_attn_kernel<T, D, NCB>, kThreads, 0) != hipSuccess || v <= 0) v = 1;
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&v, q4_attn_kernel<T, D, NCB, false>, kThreads, 0) != hipSuccess || v <= 0) v = 1;
         return v;
     }();
     return n;
@@ -656,8 +669,8 @@ int stage_floats(int cols, int d) {  // rows staged at a time: a power of two, a
     return per * d;
 }
 
-template <typename T, int D, int NCB>
-hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStream_t s) {
+template <typename T, int D, int NCB, bool WHOLE>
+hipError_t launch_w(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStream_t s) {
     Q4Ws ws{};
     if (plan.merge) {
         ws.o = static_cast<float*>(wsp);
@@ -665,14 +678,14 @@ hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStrea
         ws.runs = reinterpret_cast<int32_t*>(ws.ml + (size_t)plan.n_slots * a.cols * 2);
     }
     const int stage = stage_floats(a.cols, D);
-    const size_t lds = ring_bytes(D) + (size_t)(a.batch + 1) * 4;
+    const size_t lds = ring_bytes(D) + (plan.merge ? (size_t)(a.batch + 1) * 4 : 0);
     if (lds > (64 << 10)) {
         static std::atomic<uint64_t> on{0};
         const hipError_t e =
-            allow_lds(reinterpret_cast<const void*>(&q4_attn_kernel<T, D, NCB>), ring_bytes(D) + (kQ4MaxBatch + 1) * 4, on);
+            allow_lds(reinterpret_cast<const void*>(&q4_attn_kernel<T, D, NCB, WHOLE>), ring_bytes(D) + (kQ4MaxBatch + 1) * 4, on);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((q4_attn_kernel<T, D, NCB>), dim3(plan.grid), dim3(kThreads), lds, s, a, ws, stage);
+    hipLaunchKernelGGL((q4_attn_kernel<T, D, NCB, WHOLE>), dim3(plan.grid), dim3(kThreads), lds, s, a, ws, stage);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (plan.merge) {
@@ -685,6 +698,11 @@ hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStrea
             hipLaunchKernelGGL((q4_merge_kernel<T, 1>), dim3((a.cols * D + 63) / 64, n_seg, a.batch), dim3(256), 0, s, a, ws, D);
     }
     return hipGetLastError();
+}
+
+template <typename T, int D, int NCB>
+hipError_t launch_t(const Q4AttnArgs& a, const Q4Plan& p, void* ws, hipStream_t s) {
+    return p.merge ? launch_w<T, D, NCB, false>(a, p, ws, s) : launch_w<T, D, NCB, true>(a, p, ws, s);
 }
 
 template <typename T>
@@ -749,6 +767,7 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     a.item_pages = ip;
     p.merge = a.use_pages > ip;
     p.n_slots = (long long)a.batch * n_seg + p.grid;
+    if (!p.merge) p.grid = (int)std::min<long long>((long long)a.batch * n_seg, 1 << 20);  // as many workgroups as segments
     if ((long long)a.batch * n_seg * ((a.use_pages + ip - 1) / ip) > 0x7fffffffll || n_seg > 65535) p.grid = 0;  // the caller refuses
     p.ws_bytes = p.merge ? ((size_t)p.n_slots * a.cols * (d + 2) + (size_t)2 * a.batch * n_seg) * 4 : 0;
     return p;
