@@ -35,8 +35,6 @@ constexpr int kMaxRuns = 1024;    // runs of one segment the merge stages
 constexpr int kStage = 1024;      // most floats a wavefront stages at a time for the merge in LDS
 constexpr int kMaxSplits = 32;    // key splits of a tiled row block
 constexpr int kTileRows = 64;     // rows of a KV head past which the tiled kernel runs
-constexpr long long kWholeBytes = 160 << 10;  // of a segment's pages
-static_assert(kWholeBytes * 3 / 2 / (18 * 64) <= sched::kSubPages, "a whole segment's page ids fit one load of the lanes");
 constexpr int kAlign = 8;         // grid workgroups a segment from which segments are cut into pieces of their own
 constexpr int kItemPages = 16;    // pages of a work item
 
@@ -409,7 +407,7 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
                 int first, n_my;
                 sched::sub_pages(sub, run.pg1, wave, &first, &n_my);
                 // A page id outside the pool holds no tokens: page 0 is read in its place, all of it masked.
-                const int pid_raw = lane >= n_my ? 0 : WHOLE ? pid_first : pt[first + kWaves * lane];
+                const int pid_raw = lane >= n_my ? 0 : WHOLE && sub == 0 ? pid_first : pt[first + kWaves * lane];
                 const bool bad = !sched::page_ok(pid_raw, a.g.n_pages);
                 const int pid_v = bad ? 0 : pid_raw;
                 const uint64_t bad_pages = __ballot(bad);
@@ -758,11 +756,14 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     // 41.6 us); below, 8 lose to 16 (one of 32k, 8 KV heads: 25.8 against 22.9).
     const long long items = (long long)a.batch * n_seg * a.use_pages / kItemPages;
     int ip = items >= 2LL * p.grid && items < 8LL * p.grid ? kItemPages / 2 : kItemPages;
-    // A short segment is one item, read by one workgroup in less time than the runs of several and their merge
-    // take; one half longer counts as short where there is a segment for every CU.  (16-bit rows, 8 KV heads, D 128:
-    // 128 sequences of 992 tokens, 140 KB: 46 us cut, 38 whole; 32 of 1552, 218 KB: 26 and 19; but one sequence of
-    // that length at D 64: 16.5 and 21, and 32 of 3400, 480 KB, with the shortest a quarter of it: 28.5 and 30.)
-    const long long whole = (long long)a.batch * n_seg >= cus ? kWholeBytes * 3 / 2 : kWholeBytes;
+    // A short segment is read whole by one workgroup in less time than the runs of several and their merge take, a longer
+    // one too where segments fill the chip by themselves.  Cut against whole, 16-bit rows, us:
+    //   8 KV heads, D 128:  1 sequence of 992 tokens (140 KB) 15.9, 11.6; of 2128 (300 KB) 16.4, 18.7
+    //                       32 of 3264 (460 KB) 34.5, 29.4, the shortest a quarter as long 28.6, 28.1; of 6400 (900 KB) 39, 49
+    //                       256 of 6400 369, 335 and 248, 243; of 12800 (1800 KB) 464, 477
+    //   2 KV heads, D 256:  128 of 770 (217 KB) 32, 17; of 1632 (460 KB) 42, 27; 1024 of 3200 (900 KB) 361, 339 and 262, 242
+    const long long segs = (long long)a.batch * n_seg;
+    const long long whole = segs >= 8LL * cus ? 960 << 10 : segs >= cus ? 480 << 10 : 224 << 10;  // of a segment's pages, at most
     if ((long long)a.use_pages * q4_block_bytes(d) <= whole) ip = std::max(ip, a.use_pages);
     a.item_pages = ip;
     p.merge = a.use_pages > ip;

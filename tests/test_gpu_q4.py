@@ -702,7 +702,7 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("dtype,d,hq,hkv,n,top", [("f16", 128, 8, 2, 140, 1500), ("f32", 64, 4, 4, 70, 2000), ("bf16", 256, 16, 16, 24, 1500),
-                                                  ("f16", 64, 32, 32, 24, 4000)])
+                                                  ("f16", 64, 32, 32, 24, 4000), ("bf16", 256, 8, 8, 25, 1980), ("f16", 64, 8, 8, 32, 6500)])
 def test_decode_many_segments(dtype, d, hq, hkv, n, top):
     """A segment for every CU: whole ones up to a size, items of half the pages past it."""
     lens = np.random.default_rng(n).integers(0, top + 1, n).tolist()
