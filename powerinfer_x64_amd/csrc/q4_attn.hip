@@ -13,12 +13,16 @@
 // 16-bit output).  f32 queries and their P are split into two f16 (22 bits) and multiplied twice.  The scale is
 // applied to the f32 scores.
 //
-// Bound: a long context by HBM (18 D bytes a page and KV head); the dequantisation costs about 1.5 VALU instructions
-// a code and runs beside the loads of the next pages.  A short one by launches and round trips.
+// Bound: a long context by HBM (18 D bytes a page and KV head) with the dequantisation, about 1.5 VALU instructions
+// a code, beside it: 32 ragged sequences of 1k to 32k tokens, 32 / 8 heads, D 128, f16 102-106 us (523 MB, 5.0 TB/s, what a
+// large copy reaches; the loads alone 97-99, the arithmetic alone on pages in the L2 90); 8 of 64k, 16 / 2 heads, D 256, bf16
+// 59-60 (302 MB, 5.1 TB/s).  A few drafted tokens a sequence by the VALU, half of the SIMDs' cycles, at two wavefronts a
+// SIMD: 8 sequences of 1 to 8 rows over 2k to 16k tokens, 32 / 8 heads 36 us (97 MB, 2.7 TB/s).  A short context by a launch
+// and round trips: 512 tokens, 32 heads, f32 8.9 us.  The merge: 4 to 6 us.
 //
 // Schedule: decode_sched.hpp's items (pages of one (sequence, KV head, row block) segment), an equal contiguous range
 // to each of a persistent grid's workgroups; a segment inside one workgroup is written at once,
-// others leave (max, sum, O) for q4_merge_kernel.  Where every segment is one item the merge is not launched.
+// others leave (max, sum, O) for q4_merge_kernel.  Short segments are a workgroup each instead, and no merge follows (q4_plan).
 #include "pi_device.hpp"
 #include "q4_launch.hpp"
 

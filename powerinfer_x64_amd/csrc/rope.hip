@@ -6,7 +6,8 @@
 // reduced to a half turn in f64 and only the remainder goes to f32 (sincospi, error below 2 ulp).
 // The rotation is f32, rounded once to the rows' type.
 //
-// Bound by memory: a row is read and written once.  A workgroup takes one token (its angles are computed
+// Bound by memory: a row is read and written once (4096 tokens of 32 + 8 heads, D 128, bf16: 14 us, 84 MB at 5.9 TB/s;
+// 1000 tokens of 16 + 2 heads, D 256, f32, a quarter of it rotated: 8.7 us, 37 MB at 4.2; one token: 2.6 us, a launch).  A workgroup takes one token (its angles are computed
 // once, into LDS) and its threads 8 pairs each: two 16-byte chunks half a rotation apart (halves), or one
 // chunk (pairs); the rest of the head is copied when the output is another tensor.
 #include "pi_device.hpp"
