@@ -69,25 +69,25 @@ __device__ __forceinline__ void load_block(const char* blk, uint32_t dst, uint32
     if constexpr (D == 64)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
                      "global_load_lds_dwordx4 %1, %3\n\t"
-                     "global_load_lds_dword %2, %3 offset:1024\n\t"
+                     "global_load_lds_dword %2, %3 offset:0x400\n\t"
                      "s_mov_b32 m0, %0"
                      : "=&s"(saved) : "v"(lane16), "v"(lane4), "s"(blk), "s"(dst) : "memory");
     else if constexpr (D == 128)
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
                      "global_load_lds_dwordx4 %1, %3\n\t"
-                     "global_load_lds_dwordx4 %1, %3 offset:1024\n\t"
-                     "global_load_lds_dword %2, %3 offset:2048\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:0x400\n\t"
+                     "global_load_lds_dword %2, %3 offset:0x800\n\t"
                      "s_mov_b32 m0, %0"
                      : "=&s"(saved) : "v"(lane16), "v"(lane4), "s"(blk), "s"(dst) : "memory");
     else
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\t"
                      "global_load_lds_dwordx4 %1, %3\n\t"
-                     "global_load_lds_dwordx4 %1, %3 offset:1024\n\t"
-                     "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
-                     "global_load_lds_dwordx4 %1, %3 offset:3072\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:0x400\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:0x800\n\t"
+                     "global_load_lds_dwordx4 %1, %3 offset:0xc00\n\t"
                      "s_mov_b32 m0, %5\n\t"
                      "global_load_lds_dword %2, %6\n\t"
-                     "global_load_lds_dword %2, %6 offset:256\n\t"
+                     "global_load_lds_dword %2, %6 offset:0x100\n\t"
                      "s_mov_b32 m0, %0"
                      : "=&s"(saved) : "v"(lane16), "v"(lane4), "s"(blk), "s"(dst), "s"(dst + 4096), "s"(blk + 4096) : "memory");
 }
@@ -777,7 +777,7 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
     a.item_pages = ip;
     p.merge = a.use_pages > ip;
     p.n_slots = (long long)a.batch * n_seg + p.grid;
-    if (!p.merge) p.grid = (int)std::min<long long>((long long)a.batch * n_seg, 1 << 20);  // as many workgroups as segments
+    if (!p.merge) p.grid = (int)std::min<long long>(std::max(segs, 1ll), 1 << 20);  // as many workgroups as segments
     if ((long long)a.batch * n_seg * ((a.use_pages + ip - 1) / ip) > 0x7fffffffll || n_seg > 65535) p.grid = 0;  // the caller refuses
     p.ws_bytes = p.merge ? ((size_t)p.n_slots * a.cols * (d + 2) + (size_t)2 * a.batch * n_seg) * 4 : 0;
     return p;
