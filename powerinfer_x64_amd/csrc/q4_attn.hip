@@ -146,7 +146,7 @@ template <typename T, int D>
 struct Query {
     static constexpr int NJ = D / kQ4Group, PREC = std::is_same<T, float>::value ? 2 : 1;
     f16x8 r[PREC][NJ];
-    // returns the factor from a raw product to log2 units
+    // returns the factor from a raw product to log2 units, above 0
     __device__ __forceinline__ float load(const T* q, long long off, int grp, float scale) {
         float x[8 * NJ];
         const T* p = q + (off < 0 ? 0 : off) + 8 * grp;
@@ -165,6 +165,13 @@ struct Query {
             f = __builtin_bit_cast(float, (uint32_t)(127 - e1) << 23);
             back = ldexpf(back, e1);
         }
+        // A negative scale turns the row instead, and one of 0 stays above it (all scores as good as equal, masks -inf): the
+        // largest raw product is the largest score.
+        if (back < 0.f) {
+            f = -f;
+            back = -back;
+        }
+        if (back < 1e-30f) back = 1e-30f;
         if (off < 0) f = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
@@ -214,7 +221,6 @@ __device__ __forceinline__ void process(Acc<D, NCB>& acc, const Page<D>* pg, con
         float mx = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            s[u][cb] *= back[cb];
             if (edge) {
                 const int left = lim[cb] - tok0[u] - 4 * grp;  // tokens of the lane's four that count
 #pragma unroll
@@ -224,6 +230,7 @@ __device__ __forceinline__ void process(Acc<D, NCB>& acc, const Page<D>* pg, con
 #pragma unroll
             for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][cb][r]);
         }
+        mx *= back[cb];
         if (__any(mx > acc.m[cb] + kLazy)) {
             mx = wave_max_xor(mx, 16);
             mx = wave_max_xor(mx, 32);
@@ -239,7 +246,7 @@ __device__ __forceinline__ void process(Acc<D, NCB>& acc, const Page<D>* pg, con
         for (int u = 0; u < 2; ++u) {
             float p[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) p[r] = fast_exp2(s[u][cb][r] - acc.m[cb]);
+            for (int r = 0; r < 4; ++r) p[r] = fast_exp2(fmaf(s[u][cb][r], back[cb], -acc.m[cb]));
             sum += (p[0] + p[1]) + (p[2] + p[3]);
             const float pv[4] = {p[0], p[2], p[1], p[3]};  // the order of the V codes
 #pragma unroll
@@ -696,10 +703,10 @@ hipError_t launch_w(const Q4AttnArgs& a, const Q4Plan& plan, void* wsp, hipStrea
     if (e != hipSuccess) return e;
     if (plan.merge) {
         const int n_seg = a.g.n_kv_heads * a.n_cb;
-        // 256 values a workgroup, or 64 where that leaves few workgroups (one sequence of 32k tokens, 8 KV heads, D 128: the whole
-        // call 23.9, 23.4 us; with many 64 lose: 64 sequences of 4000 73.4, 77.4)
+        // 256 values a workgroup, or 64 where that leaves few workgroups (8 sequences of 64k, 2 KV heads, D 256: the
+        // whole step 78.2, 77.5 us; with many 64 lose: 64 sequences of 4000, 8 KV heads, D 128 73.4, 77.4)
         const long long wg4 = (long long)((a.cols * D + 255) / 256) * n_seg * a.batch;
-        if (wg4 >= 128)
+        if (wg4 >= 256)
             hipLaunchKernelGGL((q4_merge_kernel<T, 4>), dim3((a.cols * D + 255) / 256, n_seg, a.batch), dim3(256), 0, s, a, ws, D);
         else
             hipLaunchKernelGGL((q4_merge_kernel<T, 1>), dim3((a.cols * D + 63) / 64, n_seg, a.batch), dim3(256), 0, s, a, ws, D);
