@@ -564,7 +564,8 @@ __global__ __launch_bounds__(kThreads, (min_waves<T, D, NCB>())) void q4_attn_ke
 }
 
 // Joins the runs of the segments that span several workgroups' ranges and writes zeros for the rows of
-// sequences without keys.  A workgroup: 64 V values of one segment; its 4 wavefronts take every 4th run each.
+// sequences without keys.  A workgroup: 64 V values of one segment; its 4 wavefronts take every 4th run each.  A launch and two
+// trips to memory: 4 to 6 us whatever the shape, so short segments go without it.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void q4_merge_kernel(Q4AttnArgs a, Q4Ws ws, int D) {
     typedef typename std::conditional<V == 4, f32x4, float>::type VT;
