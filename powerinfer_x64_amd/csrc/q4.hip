@@ -180,7 +180,9 @@ struct Weights {
 
 // Norm and rotation of a lane's channels.  cs: cos and sin of the token's pairs.  u, v: the chunks
 // (v: VEC only).
-template <typename T, typename R, typename R2, bool VEC, int D>
+// CUT: the pairs layout's rotation may end inside a chunk (a test of every pair: 39 us for 33 for a prompt of 4096, but 34 for the
+// 42 of one chunk a lane).
+template <typename T, typename R, typename R2, bool VEC, int D, bool CUT>
 __device__ __forceinline__ void norm_rotate(const Raw<T, VEC>& raw, const Chunks& ch, const Weights& w, float eps, int half, int layout,
                                             const R2* cs, R* u, R* v) {
     typedef Real<R> F;
@@ -207,7 +209,7 @@ __device__ __forceinline__ void norm_rotate(const Raw<T, VEC>& raw, const Chunks
             if (d0 >= 2 * half) return;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-                if (!VEC && d0 + e >= 2 * half) break;
+                if (CUT && d0 + e >= 2 * half) break;
                 const R2 a = cs[(d0 + e) >> 1];
                 const R x0 = z[e], x1 = z[e + 1];
                 z[e] = x0 * a.x - x1 * a.y;
@@ -292,11 +294,11 @@ __device__ __forceinline__ void store8(T* out, const float* y) {
 }
 
 // A lane's channels of a query row: normed, rotated, written in the rows' type.
-template <typename T, bool VEC, int D>
+template <typename T, bool VEC, int D, bool CUT>
 __device__ __forceinline__ void put_q(const Q4AppendArgs& a, const Raw<T, VEC>& raw, const Weights& w, int row, int h, const Chunks& ch,
                                       const float2* cs) {
     float u[8], v[8];
-    norm_rotate<T, float, float2, VEC, D>(raw, ch, w, a.eps, a.plan.half, a.plan.layout, cs, u, v);
+    norm_rotate<T, float, float2, VEC, D, CUT>(raw, ch, w, a.eps, a.plan.half, a.plan.layout, cs, u, v);
     T* out = static_cast<T*>(a.q_out.p) + row * a.q_out.tok + h * a.q_out.head;
     store8<T, VEC>(out + ch.a, u);
     if (VEC) store8<T, VEC>(out + ch.b, v);
@@ -338,14 +340,14 @@ __device__ __forceinline__ void put_codes(const Q4AppendArgs& a, uint32_t w, flo
 }
 
 // A lane's channels of a key or value row: normed and rotated (keys), quantised, stored.
-template <typename T, bool VEC, int D>
+template <typename T, bool VEC, int D, bool CUT>
 __device__ __forceinline__ void put_kv(const Q4AppendArgs& a, const Raw<T, VEC>& raw, const Weights& nw, bool is_v, int row, int kh,
                                        const Chunks& ch, const Place& pl, const double2* cs) {
     float s0, s1 = 0.f;
     uint32_t w0, w1 = 0;
     if (!is_v) {
         double u[8], v[8];
-        norm_rotate<T, double, double2, VEC, D>(raw, ch, nw, a.eps, a.plan.half, a.plan.layout, cs, u, v);
+        norm_rotate<T, double, double2, VEC, D, CUT>(raw, ch, nw, a.eps, a.plan.half, a.plan.layout, cs, u, v);
         w0 = quantise8<double>(u, &s0);
         if (VEC) w1 = quantise8<double>(v, &s1);
     } else {
@@ -367,7 +369,7 @@ __device__ __forceinline__ void put_kv(const Q4AppendArgs& a, const Raw<T, VEC>&
 // queries of `toks` tokens (f32): in one launch, so that the heavier arithmetic runs beside the larger share
 // of the bytes.  blockIdx.y: a share of the tokens' rows.  A workgroup's first rows are requested before it looks
 // up its tokens' places and computes their angles.
-template <typename T, bool VEC, int D>
+template <typename T, bool VEC, int D, bool CUT>
 __global__ __launch_bounds__(kThreads, 3) void q4_append_kernel(Q4AppendArgs a, int toks, int kv_wgs) {
     __shared__ double2 s_cs[kTable];
     __shared__ Place s_place[kMaxToks];
@@ -436,9 +438,9 @@ __global__ __launch_bounds__(kThreads, 3) void q4_append_kernel(Q4AppendArgs a, 
         const Place pl = s_place[tn];
         if (pl.pos < 0) continue;  // a row of no sequence; uniform over a row's lanes
         if (kv)
-            put_kv<T, VEC, D>(a, now, w, vn, row0 + tn, hn, ch, pl, s_cs + tn * half);
+            put_kv<T, VEC, D, CUT>(a, now, w, vn, row0 + tn, hn, ch, pl, s_cs + tn * half);
         else
-            put_q<T, VEC, D>(a, now, w, row0 + tn, hn, ch, reinterpret_cast<const float2*>(s_cs) + tn * half);
+            put_q<T, VEC, D, CUT>(a, now, w, row0 + tn, hn, ch, reinterpret_cast<const float2*>(s_cs) + tn * half);
     }
 }
 
@@ -446,7 +448,7 @@ template <typename T, int D>
 hipError_t launch_append_d(const Q4AppendArgs& a, hipStream_t s) {
     const int e = (int)sizeof(T);
     const int half = a.plan.half;
-    bool vec = a.plan.layout == 1 && half ? half % 32 == 0 && (D - 2 * half) % 64 == 0 : half % 4 == 0;
+    bool vec = a.plan.layout == 1 && half ? half % 32 == 0 && (D - 2 * half) % 64 == 0 : true;
     for (const HeadRows* r : {&a.q, &a.q_out, &a.k, &a.v})
         if (r->p) vec = vec && reinterpret_cast<uintptr_t>(r->p) % 16 == 0 && r->tok * e % 16 == 0 && r->head * e % 16 == 0;
     // Tokens of a workgroup: as many as fill the angles' table in one pass of its threads; one while the launch is small.
@@ -457,10 +459,12 @@ hipError_t launch_append_d(const Q4AppendArgs& a, hipStream_t s) {
     const int blocks = (toks * std::max(a.q.n, 2 * a.g.n_kv_heads) + rpi - 1) / rpi;
     const int y = all * blocks <= 2048 ? std::min(blocks, 65535) : 1;
     const dim3 grid((unsigned)all, y);
-    if (vec)
-        hipLaunchKernelGGL((q4_append_kernel<T, true, D>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
+    if (vec && a.plan.layout == 0 && half % 4)
+        hipLaunchKernelGGL((q4_append_kernel<T, true, D, true>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
+    else if (vec)
+        hipLaunchKernelGGL((q4_append_kernel<T, true, D, false>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
     else
-        hipLaunchKernelGGL((q4_append_kernel<T, false, D>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
+        hipLaunchKernelGGL((q4_append_kernel<T, false, D, true>), grid, dim3(kThreads), 0, s, a, toks, (int)wgs);
     return hipGetLastError();
 }
 

@@ -103,13 +103,45 @@ __global__ __launch_bounds__(kThreads) void rope_vec_kernel(RopeArgs a, int copy
     }
 }
 
-// Any widths, strides and alignment: a thread turns one pair or copies one channel.
+// n (1 .. 8) elements at any alignment of T: eight by one wide access, which the memory takes at any address.
 template <typename T>
+__device__ __forceinline__ void load_n(const T* p, int n, float* x) {
+    typedef T t8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    if (n == 8) {
+        const t8 r = *reinterpret_cast<const t8*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f32(r[i]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? to_f32(p[i]) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store_n(T* p, int n, const float* x) {
+    typedef T t8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    if (n == 8) {
+        t8 r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = from_f32<T>(x[i]);
+        *reinterpret_cast<t8*>(p) = r;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) p[i] = from_f32<T>(x[i]);
+}
+
+// Any widths, strides and alignment: the chunks above where they lie, the last of a part with fewer channels.  (4096 tokens of
+// 32 + 8 heads, D 128, 34 channels rotated, f16: pairs 17 us, halves 35; a pair or a channel a thread took 56 and 53.)
+template <typename T, int LAYOUT>
 __global__ __launch_bounds__(kThreads) void rope_any_kernel(RopeArgs a, int copy_q, int copy_k) {
     __shared__ float2 s_cs[kMaxHalf];
     const int t = blockIdx.x, tid = threadIdx.x;
-    const int half = a.plan.half, rest = a.head_dim - 2 * half;
-    const int per_q = half + (copy_q ? rest : 0), per_k = half + (copy_k ? rest : 0);
+    const int half = a.plan.half, D = a.head_dim;
+    const int rot = LAYOUT == 1 ? (half + 7) / 8 : (half + 3) / 4;  // rotating units of a head
+    const int past = LAYOUT == 1 ? 2 * half : min(8 * rot, D);      // first channel of the units past them
+    const int rest = (D - past + 7) / 8;
+    const int per_q = rot + (copy_q ? rest : 0), per_k = rot + (copy_k ? rest : 0);
     const int nq = a.in[0].n * per_q, units = nq + a.in[1].n * per_k;
     const double pos = a.pos[t];
     if (tid < half) s_cs[tid] = angle_f32(pos, a.plan.turns[tid], (float)a.plan.mscale);
@@ -120,15 +152,36 @@ __global__ __launch_bounds__(kThreads) void rope_any_kernel(RopeArgs a, int copy
         const int h = v / per, c = v - h * per;
         const T* in = static_cast<const T*>(a.in[w].p) + t * a.in[w].tok + h * a.in[w].head;
         T* out = static_cast<T*>(a.out[w].p) + t * a.out[w].tok + h * a.out[w].head;
-        if (c >= half) {
-            out[half + c] = in[half + c];
-            continue;
+        float x[8], y[8];
+        if (c >= rot) {
+            const int d = past + 8 * (c - rot), n = min(8, D - d);
+            load_n(in + d, n, x);
+            store_n(out + d, n, x);
+        } else if (LAYOUT == 1) {
+            const int n = min(8, half - 8 * c);
+            float x1[8], y1[8];
+            load_n(in + 8 * c, n, x);
+            load_n(in + half + 8 * c, n, x1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 cs = s_cs[min(8 * c + i, half - 1)];
+                y[i] = x[i] * cs.x - x1[i] * cs.y;
+                y1[i] = x[i] * cs.y + x1[i] * cs.x;
+            }
+            store_n(out + 8 * c, n, y);
+            store_n(out + half + 8 * c, n, y1);
+        } else {
+            const int n = min(8, D - 8 * c);
+            load_n(in + 8 * c, n, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool on = 4 * c + i < half;  // else channels past the rotation
+                const float2 cs = s_cs[min(4 * c + i, half - 1)];
+                y[2 * i] = on ? x[2 * i] * cs.x - x[2 * i + 1] * cs.y : x[2 * i];
+                y[2 * i + 1] = on ? x[2 * i] * cs.y + x[2 * i + 1] * cs.x : x[2 * i + 1];
+            }
+            store_n(out + 8 * c, n, y);
         }
-        const int d0 = a.plan.layout == 1 ? c : 2 * c, d1 = a.plan.layout == 1 ? c + half : 2 * c + 1;
-        const float x0 = to_f32(in[d0]), x1 = to_f32(in[d1]);
-        const float2 cs = s_cs[c];
-        out[d0] = from_f32<T>(x0 * cs.x - x1 * cs.y);
-        out[d1] = from_f32<T>(x0 * cs.y + x1 * cs.x);
     }
 }
 
@@ -142,7 +195,7 @@ hipError_t launch_t(const RopeArgs& a, hipStream_t s) {
             vec = vec && reinterpret_cast<uintptr_t>(r->p) % 16 == 0 && r->tok * e % 16 == 0 && r->head * e % 16 == 0;
     }
     const int copy_q = a.out[0].p != a.in[0].p, copy_k = a.out[1].p != a.in[1].p;
-    const int per = vec ? (a.plan.layout == 1 ? half / 8 : half / 4) + (a.head_dim - 2 * half) / 8 : a.head_dim - half;
+    const int per = a.plan.layout == 1 ? (half + 7) / 8 + (a.head_dim - 2 * half + 7) / 8 : (a.head_dim + 7) / 8;
     const int blocks = std::max(1, (per * (a.in[0].n + a.in[1].n) + kThreads - 1) / kThreads);
     // One pass of a token's rows a workgroup while that does not fill the chip, else a workgroup a token.
     const int y = (long long)a.n_tok * blocks <= 2048 ? std::min(blocks, 65535) : 1;
@@ -151,8 +204,10 @@ hipError_t launch_t(const RopeArgs& a, hipStream_t s) {
         hipLaunchKernelGGL((rope_vec_kernel<T, 1>), grid, dim3(kThreads), 0, s, a, copy_q, copy_k);
     else if (vec)
         hipLaunchKernelGGL((rope_vec_kernel<T, 0>), grid, dim3(kThreads), 0, s, a, copy_q, copy_k);
+    else if (a.plan.layout == 1)
+        hipLaunchKernelGGL((rope_any_kernel<T, 1>), grid, dim3(kThreads), 0, s, a, copy_q, copy_k);
     else
-        hipLaunchKernelGGL((rope_any_kernel<T>), grid, dim3(kThreads), 0, s, a, copy_q, copy_k);
+        hipLaunchKernelGGL((rope_any_kernel<T, 0>), grid, dim3(kThreads), 0, s, a, copy_q, copy_k);
     return hipGetLastError();
 }
 

@@ -755,3 +755,25 @@ def test_closed_plans_shared_outputs_and_sizes_are_refused():
                                 None, None, dev.stream()) == unsupported
     need = ctypes.c_size_t()
     assert dev.lib.pi_q4_attn_ws_bytes(dev.h, pool.p, rt.F16, 1 << 30, 4096, 1 << 30, 4, 0, 8, 0, ctypes.byref(need)) == unsupported
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("layout", ["pairs", "halves"])
+@pytest.mark.parametrize("d,rope_dim", [(67, 22), (20, 20), (13, 6), (7, 2), (128, 34), (250, 250)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_rope_odd_widths_between_guards(dtype, layout, d, rope_dim, in_place):
+    """Chunks that end before their eighth channel, rows at odd offsets: nothing beside the rows is written."""
+    dev, rng = device(), np.random.default_rng(d + rope_dim)
+    plan = rt.RopePlan(dev, rope_dim, base=1e4, layout=layout)
+    n, h, gap = 9, 3, 5
+    src = normal(rng, n * h * (d + gap) + 1, dtype=dtype)
+    dst = src.clone() if in_place else torch.full_like(src, 9.0)
+    rows = lambda t: t[1:].view(n, h, d + gap)[..., :d]  # noqa: E731
+    pos = rng.integers(0, 5000, n)
+    rt.rope_apply(dev, plan, rows(dst if in_place else src), None, i32(pos), rows(dst))
+    want = ref.rotate(f64(rows(src)), pos, plan.freqs, 1.0, layout)
+    assert (np.abs(f64(rows(dst)) - want) <= rotation_tol(f64(rows(src)), 1.0, dtype)(want)).all()
+    assert torch.equal(rows(dst)[..., rope_dim:], rows(src)[..., rope_dim:])
+    between = lambda t: t[1:].view(n, h, d + gap)[..., d:]  # noqa: E731
+    assert dst[0] == (src[0] if in_place else 9.0)
+    assert torch.equal(between(dst), between(src)) if in_place else (between(dst) == 9.0).all()
