@@ -748,7 +748,10 @@ Q4Plan q4_plan(Q4AttnArgs& a, int device) {
         // Few row blocks: their keys are split while that fills idle CUs and each part keeps 4 tiles.  (40 rows over 16000 keys,
         // 32 / 8 heads, D 128: 8 parts 67 us, 32 35.  Parts of 2 tiles: a prompt of 512 at D 64 16.2, 17.5 us, at D 128 29.2,
         // 29.5, at D 256 34.0, 32.0; more parts than CUs: three prompts of 300 to 1200 at D 64 24.1, 29.0.)
-        long long splits = wgs >= cus ? 1 : std::min<long long>({kMaxSplits, cus / wgs, a.use_pages / 16});
+        // Of a ragged batch's row blocks no more exist than its rows fill, and one more a sequence.  (7 chunks of up to 349 tokens
+        // over up to 6900, f32 D 256, 5 / 1 heads: 264 us with the grid's count, 148 with this.)
+        const long long blocks = n_kv * std::min<long long>(n_blk * a.batch, (long long)a.n_rows * a.group / per + a.batch);
+        long long splits = std::min<long long>({kMaxSplits, cus / blocks, a.use_pages / 16});
         splits = std::max<long long>(splits, 1);
         // (a merge of mostly rows of no sequence may be more threads than a launch takes)
         if ((long long)a.n_rows * a.n_q_heads * (d / 4) >= 1ll << 32) splits = 1;
